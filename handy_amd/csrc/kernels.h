@@ -1,6 +1,7 @@
 // Host-callable launchers of the HIP kernels (one translation unit per k_*.hip file).
 #pragma once
 #include "wmi_common.h"
+#include "../../include/wmi.h"
 
 namespace wmi {
 
@@ -126,5 +127,32 @@ bool splitk_residual_ln(float *x, const float *ws, int splits, const float *bias
                         const int *gather, int n_out, hipStream_t st);         // x[m] += sum + bias; out[i] = LN(x[gather ? gather[i] : i])
 bool splitk_f16(const float *ws, int splits, const float *bias, int gelu, float scale, f16 *out, int M, int N, hipStream_t st);
 bool splitk_dec_qkv(const float *ws, int splits, const float *bias, const DecRow *rows, int M, int d, int H, f16 *q, f16 *kc, f16 *vc, hipStream_t st);
+
+
+// ---- k_paged.hip : attention of new tokens over a paged cache (the operator behind wmi_paged_attention) ----------------------
+struct PagedAttn {
+    const void *k, *v, *q;
+    void *out;
+    const int *table, *cu, *kv_lens;                              // [n_seq][table_stride], [n_seq + 1], [n_seq]
+    long page_stride, token_stride, head_stride, q_row, q_head, o_row, o_head, table_stride;   // elements
+    float scale;
+    int dtype, dim, hkv, group, lp, n_pages, cols, n_seq, n_rows, window, max_new, max_kv;     // lp: log2 of a page's tokens
+};
+size_t paged_attention_workspace(const PagedAttn &a);
+bool paged_attention(const PagedAttn &a, void *workspace, hipStream_t st);
+
+// ---- k_draw.hip : one token a row from its logits (the operator behind wmi_sample_tokens) ------------------------------------
+struct DrawArgs {
+    const void *logits;
+    const float *temperature, *top_p, *min_p;                    // null: 1, off, off
+    const float *uniform;
+    const int *top_k;                                             // null: off
+    int *token;
+    float *logprob;                                               // null: not wanted
+    long row_stride;
+    int n_rows, n_vocab, dtype;
+};
+constexpr int kDrawMaxVocab = 262144;
+bool draw_tokens(const DrawArgs &a, hipStream_t st);
 
 }  // namespace wmi

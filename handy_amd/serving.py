@@ -1,0 +1,233 @@
+"""Serving operators over a paged K/V cache, for callers that run a text decoder of their own next to the transcription: the
+step's block tables and slots (`plan_pages`), the new tokens' K and V (`write_kv`), attention of the new tokens over the cache
+(`paged_attention`) and the draw of the next token (`sample_tokens`), through the C ABI of libwhisper_mi355.so (include/wmi.h).
+No counterpart in the reference, whose engine keeps one sequence at a time.
+
+Arguments are device arrays: anything with `data_ptr()`, `shape`, `stride()` and `dtype` -- a torch tensor on the GPU, or a
+`DeviceArray` in memory of the HIP runtime the library is linked against. (In a process that uses torch, import torch before the
+library is loaded, so that both use one runtime.) Calls enqueue on `stream` (a hipStream_t value; 0 = the null stream) and return
+without waiting; outputs are the caller's buffers, so calls can be captured into graphs. Wrong arguments raise ValueError before
+anything is enqueued."""
+import ctypes as C
+import math
+from typing import NamedTuple, Optional
+
+import numpy as np
+
+from . import whisper_rs as wr
+
+_DTYPES = {"float16": 0, "bfloat16": 1, "float32": 2}
+_SIZES = {"float16": 2, "bfloat16": 2, "float32": 4, "int32": 4, "uint8": 1}
+_NUMPY = {"float16": np.float16, "bfloat16": np.uint16, "float32": np.float32, "int32": np.int32, "uint8": np.uint8}
+
+
+class DeviceArray:
+    """Array in device memory on the current HIP device. bfloat16 travels to and from the host as uint16 bit patterns."""
+
+    def __init__(self, shape, dtype: str, _base=None, _strides=None, _offset: int = 0):
+        self.shape = tuple(int(s) for s in (shape if isinstance(shape, (tuple, list)) else (shape,)))
+        self.dtype = dtype
+        self._strides = tuple(_strides) if _strides is not None else _contiguous(self.shape)
+        self._base, self._offset, self._ptr = _base, _offset, None
+        if _base is None:
+            self._bytes = math.prod(self.shape) * _SIZES[dtype]
+            self._ptr = wr.load_library().wmi_dev_alloc(max(self._bytes, 16))
+            if not self._ptr:
+                raise wr.WhisperError(f"device allocation of {self._bytes} bytes failed")
+
+    @classmethod
+    def from_numpy(cls, a, dtype: Optional[str] = None):
+        a = np.ascontiguousarray(a)
+        d = cls(a.shape, dtype or a.dtype.name)
+        if a.dtype != _NUMPY[d.dtype]:
+            raise ValueError(f"{a.dtype} is not the host form of {d.dtype}")
+        if a.size and wr.load_library().wmi_dev_upload(d.data_ptr(), a.ctypes.data, a.nbytes) != 0:
+            raise wr.WhisperError("hipMemcpy to the device failed")
+        return d
+
+    def numpy(self) -> np.ndarray:
+        """The whole array on the host (waits for the null stream's work); views copy their base and pick on the host."""
+        if self._base is not None:
+            flat = self._base.numpy().reshape(-1)[self._offset:]
+            return np.lib.stride_tricks.as_strided(flat, self.shape, [s * flat.itemsize for s in self._strides]).copy()
+        out = np.empty(self.shape, _NUMPY[self.dtype])
+        if out.size and wr.load_library().wmi_dev_download(out.ctypes.data, self._ptr, out.nbytes) != 0:
+            raise wr.WhisperError("hipMemcpy from the device failed")
+        return out
+
+    def view(self, shape, strides, offset: int = 0):
+        """Another shape over the same memory; strides and offset in elements."""
+        root = self._base or self
+        last = self._offset + offset + sum((s - 1) * t for s, t in zip(shape, strides))
+        if min(strides, default=0) < 0 or (0 not in shape and last >= math.prod(root.shape)):
+            raise ValueError("view outside the array")
+        return DeviceArray(shape, self.dtype, root, strides, self._offset + offset)
+
+    def permute(self, *order):
+        return self.view([self.shape[i] for i in order], [self._strides[i] for i in order])
+
+    def data_ptr(self): return self._ptr if self._base is None else self._base.data_ptr() + self._offset * _SIZES[self.dtype]
+    def stride(self): return self._strides
+    def numel(self): return math.prod(self.shape)
+
+    def free(self):
+        if self._ptr:
+            wr.load_library().wmi_dev_free(self._ptr)
+            self._ptr = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def _contiguous(shape):
+    out, n = [], 1
+    for s in reversed(shape):
+        out.append(n)
+        n *= s
+    return tuple(reversed(out))
+
+
+def _dtype(x) -> str:
+    d = x.dtype
+    return d if type(d) is str else str(d).replace("torch.", "")
+
+
+def _flat(x, dtype: str, n: int, name: str):
+    """pointer of a contiguous 1-d array of at least n elements"""
+    if _dtype(x) != dtype or len(x.shape) != 1 or x.shape[0] < n or (n > 1 and x.stride()[0] != 1):
+        raise ValueError(f"{name}: expected a contiguous {dtype} array of {n}")
+    return x.data_ptr() if n else None
+
+
+def _rows(x, shape, dtype: str, name: str):
+    """pointer and the two outer strides of a [rows][heads][dim] array with contiguous heads"""
+    st = x.stride()
+    if _dtype(x) != dtype or tuple(x.shape) != shape or (shape[2] > 1 and st[2] != 1):
+        raise ValueError(f"{name}: expected {dtype} {shape} with contiguous last axis")
+    return x.data_ptr(), st[0], st[1]
+
+
+def _check(rc: int, what: str):
+    if rc in (-1, -2, -3):
+        raise ValueError(what + {-1: ": bad arguments (sizes, alignment, or memory that is not the call's GPU's)", -2: ": workspace too small",
+                                 -3: ": sizes not supported"}[rc])
+    if rc != 0:
+        raise wr.WhisperError(f"{what} failed", rc)
+
+
+class PagedCache:
+    """One layer's K and V in pages: two arrays of shape [n_pages, page_tokens, n_kv_heads, head_dim], any strides with a contiguous last
+    axis and the same for both (a head-major cache is passed as its permuted view). Keeps the arrays."""
+
+    def __init__(self, k, v):
+        dt = _dtype(k)
+        if dt not in ("float16", "bfloat16") or _dtype(v) != dt:
+            raise ValueError("K and V: float16 or bfloat16, both the same")
+        if len(k.shape) != 4 or tuple(k.shape) != tuple(v.shape) or tuple(k.stride()) != tuple(v.stride()) or (k.shape[3] > 1 and k.stride()[3] != 1):
+            raise ValueError("K and V: [n_pages, page_tokens, n_kv_heads, head_dim] with the same strides and a contiguous last axis")
+        self.k, self.v, self.dtype = k, v, dt
+        self.n_pages, self.page_tokens, self.n_kv_heads, self.head_dim = (int(n) for n in k.shape)
+        st = k.stride()
+        self.c = wr.wmi_paged_cache(k.data_ptr(), v.data_ptr(), _DTYPES[dt], self.n_pages, self.page_tokens, self.n_kv_heads, self.head_dim, st[0], st[1], st[2])
+        self.ref = C.byref(self.c)
+
+
+class PagePlan(NamedTuple):
+    """Buffers of one step's plan, int32: cu_q[n_seq + 1], kv_lens[n_seq], slots[rows], positions[rows], counts[4]."""
+    cu_q: object
+    kv_lens: object
+    slots: object
+    positions: object
+    counts: object
+
+    @classmethod
+    def allocate(cls, n_seq: int, n_rows: int):
+        return cls(*(DeviceArray(n, "int32") for n in (n_seq + 1, n_seq, n_rows, n_rows, 4)))
+
+
+def plan_pages(ctx_lens, new_lens, free_pages, block_table, page_tokens: int, out: PagePlan, stream: int = 0) -> PagePlan:
+    """Admit requests in order, give them fresh pages from the front of free_pages (entered in block_table[n_seq, cols]) and number
+    their rows: see wmi_paged_plan in include/wmi.h. The number of rows planned for is the length of out.slots."""
+    n_seq, cap = int(ctx_lens.shape[0]), int(out.slots.shape[0])
+    if _dtype(block_table) != "int32" or len(block_table.shape) != 2 or block_table.shape[0] != n_seq or (block_table.shape[1] > 1 and block_table.stride()[1] != 1):
+        raise ValueError("block_table: expected int32 [n_seq, cols] with contiguous rows")
+    cols, n_free = int(block_table.shape[1]), int(free_pages.shape[0])
+    rc = wr.load_library().wmi_paged_plan(
+        _flat(ctx_lens, "int32", n_seq, "ctx_lens"), _flat(new_lens, "int32", n_seq, "new_lens"), n_seq, _flat(free_pages, "int32", n_free, "free_pages"), n_free,
+        page_tokens, block_table.data_ptr() if n_seq and cols else None, cols, max(block_table.stride()[0], cols), _flat(out.cu_q, "int32", n_seq + 1, "cu_q"),
+        _flat(out.kv_lens, "int32", n_seq, "kv_lens"), _flat(out.slots, "int32", cap, "slots"), _flat(out.positions, "int32", cap, "positions"), cap,
+        _flat(out.counts, "int32", 4, "counts"), stream)
+    if rc:
+        _check(rc, "plan_pages")
+    return out
+
+
+def write_kv(cache: PagedCache, k_new, v_new, slots, stream: int = 0) -> None:
+    """cache[slots[r]] = k_new[r], v_new[r] (rows [n_kv_heads, head_dim], any row and head strides); rows with a slot outside the cache
+    are skipped. The slots of one call must be distinct."""
+    n = int(k_new.shape[0])
+    shape = (n, cache.n_kv_heads, cache.head_dim)
+    kp, kr, kh = _rows(k_new, shape, cache.dtype, "k_new")
+    vp, vr, vh = _rows(v_new, shape, cache.dtype, "v_new")
+    rc = wr.load_library().wmi_paged_write(cache.ref, kp if n else None, kr, kh, vp if n else None, vr, vh, _flat(slots, "int32", n, "slots"), n, stream)
+    if rc:
+        _check(rc, "write_kv")
+
+
+def paged_attention_workspace(cache: PagedCache, n_rows: int, n_q_heads: int, n_seq: int, max_new: int = 0, max_kv: int = 0) -> int:
+    """Bytes of device memory `paged_attention` needs for these sizes (0: none)."""
+    a = wr.wmi_paged_attn(None, None, None, None, None, 0, 0, 0, 0, 0, 0, n_rows, n_seq, n_q_heads, 0, max_new, max_kv, 1.0)
+    need = wr.load_library().wmi_paged_attention_workspace(cache.ref, C.byref(a))
+    if need < 0:
+        _check(int(need), "paged_attention_workspace")
+    return int(need)
+
+
+def paged_attention(q, cache: PagedCache, block_table, cu_q, kv_lens, max_new: int, max_kv: int, out, scale: Optional[float] = None, window: int = 0,
+                    workspace=None, stream: int = 0):
+    """softmax(scale q K^T) V of the requests' new tokens (q and out: [n_rows, n_q_heads, head_dim]) over the cache, causal, with window
+    > 0 over the last `window` keys only: see wmi_paged_attention in include/wmi.h. max_new / max_kv: the longest request's new and
+    total tokens (0: not known; they steer the split of the work). workspace: uint8 device array of `paged_attention_workspace`
+    bytes, one for each call that may run at the same time. Returns out."""
+    shape = tuple(q.shape)
+    if len(shape) != 3 or shape[2] != cache.head_dim:
+        raise ValueError("q: expected [n_rows, n_q_heads, head_dim]")
+    qp, qr, qh = _rows(q, shape, cache.dtype, "q")
+    op, orow, oh = _rows(out, shape, cache.dtype, "out")
+    n_seq = int(kv_lens.shape[0])
+    bt = block_table
+    if _dtype(bt) != "int32" or len(bt.shape) != 2 or bt.shape[0] != n_seq or (bt.shape[1] > 1 and bt.stride()[1] != 1):
+        raise ValueError("block_table: expected int32 [n_seq, cols] with contiguous rows")
+    cols = int(bt.shape[1])
+    a = wr.wmi_paged_attn(qp, op, bt.data_ptr() if cols else None, _flat(cu_q, "int32", n_seq + 1, "cu_q"), _flat(kv_lens, "int32", n_seq, "kv_lens"), qr, qh, orow, oh,
+                          max(bt.stride()[0], cols), cols, shape[0], n_seq, shape[1], window, max_new, max_kv, cache.head_dim ** -0.5 if scale is None else scale)
+    ws, ws_bytes = None, 0
+    if workspace is not None:
+        if _dtype(workspace) != "uint8":
+            raise ValueError("workspace: expected a uint8 array")
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel()
+    rc = wr.load_library().wmi_paged_attention(cache.ref, C.byref(a), ws, ws_bytes, stream)
+    if rc:
+        _check(rc, "paged_attention")
+    return out
+
+
+def sample_tokens(logits, uniform, token, logprob=None, temperature=None, top_k=None, top_p=None, min_p=None, stream: int = 0):
+    """One token a row of logits [n_rows, n_vocab] (float32, float16 or bfloat16) into token (int32), from uniform numbers in [0, 1) (float32,
+    one a row): see wmi_sample_tokens in include/wmi.h. temperature, top_p, min_p (float32) and top_k (int32) are per row or None.
+    logprob (float32, may be None): the token's log-probability before the filters. Returns token."""
+    dt = _dtype(logits)
+    if dt not in _DTYPES or len(logits.shape) != 2 or (logits.shape[1] > 1 and logits.stride()[1] != 1):
+        raise ValueError("logits: expected float32, float16 or bfloat16 [n_rows, n_vocab] with contiguous rows")
+    n, v = int(logits.shape[0]), int(logits.shape[1])
+    opt = lambda x, d, name: None if x is None else _flat(x, d, n, name)
+    rc = wr.load_library().wmi_sample_tokens(
+        logits.data_ptr() if n else None, _DTYPES[dt], logits.stride()[0], n, v, _flat(uniform, "float32", n, "uniform"), opt(temperature, "float32", "temperature"),
+        opt(top_k, "int32", "top_k"), opt(top_p, "float32", "top_p"), opt(min_p, "float32", "min_p"), _flat(token, "int32", n, "token"),
+        opt(logprob, "float32", "logprob"), stream)
+    if rc:
+        _check(rc, "sample_tokens")
+    return token

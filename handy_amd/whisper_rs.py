@@ -97,6 +97,20 @@ class wmi_kernel_stat(C.Structure):
     _fields_ = [("ms", C.c_double), ("work", C.c_double), ("launches", C.c_longlong)]
 
 
+class wmi_paged_cache(C.Structure):
+    """include/wmi.h: one layer's paged K/V cache in device memory (strides in elements)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("n_pages", C.c_int), ("page_tokens", C.c_int), ("n_kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("page_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class wmi_paged_attn(C.Structure):
+    """include/wmi.h: one attention call over a paged cache."""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("block_table", C.c_void_p), ("cu_q", C.c_void_p), ("kv_lens", C.c_void_p),
+                ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64), ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("table_stride", C.c_int64), ("table_cols", C.c_int), ("n_rows", C.c_int), ("n_seq", C.c_int), ("n_q_heads", C.c_int),
+                ("window", C.c_int), ("max_new", C.c_int), ("max_kv", C.c_int), ("scale", C.c_float)]
+
+
 KERNEL_CLASSES = ["mel", "enc_gemm", "enc_attn", "enc_other", "dec_gemm", "dec_cross_attn", "dec_other"]
 
 # every symbol include/whisper.h and include/wmi.h declare (checked by the CPU test-suite)
@@ -135,6 +149,7 @@ wmi_batch_segment_text wmi_batch_n_tokens wmi_batch_token_data wmi_batch_lang_id
 wmi_set_force_tokens wmi_set_beam_candidates_sampled wmi_mel_batch_device wmi_mel_batch_device_normalized wmi_pcm_to_mel_device_noalloc wmi_get_mel wmi_get_encoder_output wmi_get_cross_kv
 wmi_decode_logits_all wmi_debug_gemm wmi_debug_gemm_gelu wmi_debug_expand_blocks wmi_debug_quant_rows wmi_debug_enc_attention wmi_set_window_cache wmi_get_window_cache_stats wmi_set_pipeline_groups wmi_set_encoder_lanes wmi_set_profiling wmi_set_profiling_classes wmi_get_kernel_stats wmi_reset_kernel_stats wmi_get_host_timings wmi_set_quant_decode wmi_set_quant_resident wmi_set_decoder_lanes wmi_set_pass_graphs wmi_version
 wmi_ingest_n_frames wmi_ingest_resample wmi_ingest_gate_plan wmi_ingest_gather
+wmi_paged_plan wmi_paged_write wmi_paged_attention_workspace wmi_paged_attention wmi_sample_tokens
 wmi_ctx_for_device wmi_node_init wmi_node_free wmi_node_n_devices wmi_node_state wmi_node_context wmi_node_run wmi_node_last_gather
 wmi_node_last_batches wmi_node_run_custom
 wmi_dev_alloc wmi_dev_free wmi_dev_upload wmi_dev_download wmi_dev_memset wmi_dev_sync wmi_dev_free_bytes wmi_dev_stream_create
@@ -250,6 +265,12 @@ def load_library(path: Optional[str] = None):
     L.wmi_dev_stream_create.restype = vp; L.wmi_dev_stream_create.argtypes = []
     L.wmi_dev_stream_sync.restype = ci; L.wmi_dev_stream_sync.argtypes = [vp]
     L.wmi_dev_stream_destroy.restype = None; L.wmi_dev_stream_destroy.argtypes = [vp]
+    cache_p, attn_p = C.POINTER(wmi_paged_cache), C.POINTER(wmi_paged_attn)
+    L.wmi_paged_plan.restype = ci; L.wmi_paged_plan.argtypes = [vp, vp, ci, vp, ci, ci, vp, ci, ll, vp, vp, vp, vp, ci, vp, vp]
+    L.wmi_paged_write.restype = ci; L.wmi_paged_write.argtypes = [cache_p, vp, ll, ll, vp, ll, ll, vp, ci, vp]
+    L.wmi_paged_attention_workspace.restype = ll; L.wmi_paged_attention_workspace.argtypes = [cache_p, attn_p]
+    L.wmi_paged_attention.restype = ci; L.wmi_paged_attention.argtypes = [cache_p, attn_p, vp, sz, vp]
+    L.wmi_sample_tokens.restype = ci; L.wmi_sample_tokens.argtypes = [vp, ci, ll, ci, ci, vp, vp, vp, vp, vp, vp, vp, vp]
     if path is None:
         _lib = L
     return L

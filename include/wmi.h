@@ -241,6 +241,95 @@ typedef int (*wmi_node_batch_fn)(void *user, int worker, int first, int count, w
 WHISPER_API int wmi_node_run_custom(int n_workers, int n_utts, int batch, wmi_node_batch_fn fn, void *user, wmi_node_record *records_out,
                                     int *batches_per_worker);
 
+/* ---- Serving operators: a paged K/V cache and the draw of the next token ------------------------------------------------------
+ * The pieces of a batched decoding loop for callers that run their own decoder next to the transcription: plan the step's
+ * pages, write the new tokens' K and V, attend over the cache, draw. No counterpart in the reference (its engine keeps one
+ * sequence at a time and samples on the CPU). All pointers but the two descriptions are device memory of the call's GPU: the one
+ * `stream` (a hipStream_t) belongs to, or with NULL (the null stream) the calling thread's current one; host memory or another
+ * GPU's is refused. Everything is enqueued on `stream`; nothing waits, allocates or keeps state, so calls may be captured into
+ * graphs and made from several threads. Strides count elements. 0 ok, -1 bad arguments, -2 workspace too small, -3 sizes not
+ * supported, -4 HIP error; a call that is refused does nothing. */
+enum wmi_dtype { WMI_F16 = 0, WMI_BF16 = 1, WMI_F32 = 2 };
+
+/* K and V of one layer: element e of token t of page p, head h at k + p * page_stride + t * token_stride + h * head_stride + e,
+ * and the same for v. page_tokens: a power of two up to 1024; n_pages * page_tokens < 2^31. */
+typedef struct wmi_paged_cache {
+    void *k;
+    void *v;
+    int dtype;                 /* WMI_F16 or WMI_BF16 */
+    int n_pages;
+    int page_tokens;
+    int n_kv_heads;
+    int head_dim;
+    int64_t page_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+} wmi_paged_cache;
+
+/* Block table and slot map of one step from the requests' lengths. Request i has ctx_lens[i] tokens in the cache and
+ * new_lens[i] to come; its row of block_table[n_seq][table_stride] names the pages of the cached ones. Requests are admitted in
+ * order: fresh pages are taken from the front of free_pages[n_free] and written into the rows' next entries, rows are numbered
+ * from 0. The first request that does not fit (pages or n_rows_cap rows) and all after it get nothing in this step. A request with
+ * a negative length, or longer than its table row, is passed over (0 rows, kv_lens 0).
+ *   cu_q[n_seq + 1]   first row of each request          kv_lens[n_seq]   cached + admitted new tokens
+ *   slots[n_rows_cap] page * page_tokens + offset of each row; -1 past the last row, and where the table names no page
+ *   positions[n_rows_cap]  position of each row in its sequence (0 past the last)
+ *   counts[4]         {requests admitted (index of the first that was not), rows, fresh pages taken, requests passed over}
+ * Entries of block_table that no fresh page goes to are left as they are; the call may be repeated on its own result.
+ * n_seq <= 16384. */
+WHISPER_API int wmi_paged_plan(const int *ctx_lens, const int *new_lens, int n_seq, const int *free_pages, int n_free, int page_tokens, int *block_table,
+                               int table_cols, long long table_stride, int *cu_q, int *kv_lens, int *slots, int *positions, int n_rows_cap, int *counts, void *stream);
+
+/* cache[slots[r]] = (k_new, v_new)[r], rows [n_kv_heads][head_dim] at the given strides in the cache's type; a row whose slot
+ * is negative or past the cache is skipped. The slots of one call must be distinct. */
+WHISPER_API int wmi_paged_write(const wmi_paged_cache *cache, const void *k_new, long long k_row_stride, long long k_head_stride, const void *v_new,
+                                long long v_row_stride, long long v_head_stride, const int *slots, int n_rows, void *stream);
+
+/* softmax(scale q K^T) V of n_rows query rows over the cache. Request i owns rows cu_q[i] .. cu_q[i + 1] - 1, the last of its
+ * kv_lens[i] tokens: row t of n stands at position kv_lens[i] - n + t and sees the keys up to its own position, with window > 0
+ * only the last `window` of them. Query heads share key heads in runs of n_q_heads / n_kv_heads (<= 128). Keys on pages that the
+ * cache does not have (table entry negative or >= n_pages) are left out; a row that sees no key gives zeros; rows past
+ * cu_q[n_seq] are left as they are. head_dim a multiple of 8 up to 128; 16-byte aligned pointers, strides multiples of 8.
+ * max_new and max_kv: the longest request's new and total tokens, as far as the caller knows (they steer how the work is split,
+ * larger or smaller values change no result beyond rounding; 0: not known). Scores, softmax and sums are 32-bit; the
+ * probabilities are rounded to the cache's type for the product with V. */
+typedef struct wmi_paged_attn {
+    const void *q;             /* [n_rows][n_q_heads][head_dim], the cache's type */
+    void *out;                 /* the same shape and type */
+    const int *block_table;
+    const int *cu_q;
+    const int *kv_lens;
+    int64_t q_row_stride;
+    int64_t q_head_stride;
+    int64_t out_row_stride;
+    int64_t out_head_stride;
+    int64_t table_stride;
+    int table_cols;
+    int n_rows;
+    int n_seq;
+    int n_q_heads;
+    int window;
+    int max_new;
+    int max_kv;
+    float scale;
+} wmi_paged_attn;
+/* Bytes of device memory wmi_paged_attention needs for these sizes (pointers are not looked at; 0: none), or a negative code.
+ * A workspace belongs to one call at a time: calls that may run at once, and captured graphs that may, need one each. */
+WHISPER_API long long wmi_paged_attention_workspace(const wmi_paged_cache *cache, const wmi_paged_attn *args);
+WHISPER_API int wmi_paged_attention(const wmi_paged_cache *cache, const wmi_paged_attn *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/* One token a row of logits[n_rows][n_vocab] (dtype F32, F16 or BF16, row_stride apart). With x / temperature as the
+ * distribution's logarithm, the tokens are ordered by x, equal ones by index, and kept while their rank is below top_k, the mass
+ * before them is below top_p times the mass of the first top_k, and their probability is at least min_p times the largest; the
+ * first is always kept. The token is the first, in the vocabulary's order, at which the running mass of the kept ones exceeds
+ * uniform (in [0, 1); NaN and less count as 0, more as 1 - 2^-24) times their whole mass. temperature <= 0: the most probable token (lowest index). A parameter array may be
+ * NULL (temperature 1, filter off); per row top_k <= 0, top_p >= 1, min_p <= 0 turn a filter off. -infinity and NaN are never
+ * drawn; a row with nothing to draw gives token -1. logprob (may be NULL): logarithm of the token's probability at this
+ * temperature (at 1 when temperature <= 0) before the filters. Masses are sums in 64-bit whole numbers: the result does not
+ * depend on anything but the row. n_vocab <= 262144. */
+WHISPER_API int wmi_sample_tokens(const void *logits, int dtype, long long row_stride, int n_rows, int n_vocab, const float *uniform, const float *temperature,
+                                  const int *top_k, const float *top_p, const float *min_p, int *token, float *logprob, void *stream);
+
 WHISPER_API const char *wmi_version(void);
 
 #ifdef __cplusplus

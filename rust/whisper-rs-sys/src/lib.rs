@@ -131,6 +131,51 @@ pub struct whisper_full_params {
     pub grammar_penalty: c_float,
 }
 
+/// wmi.h: element types of the serving operators' buffers
+pub const WMI_F16: c_int = 0;
+pub const WMI_BF16: c_int = 1;
+pub const WMI_F32: c_int = 2;
+
+/// wmi.h: one layer's paged K/V cache in device memory (strides in elements)
+#[repr(C)]
+#[derive(Debug, Copy, Clone)]
+pub struct wmi_paged_cache {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub dtype: c_int,
+    pub n_pages: c_int,
+    pub page_tokens: c_int,
+    pub n_kv_heads: c_int,
+    pub head_dim: c_int,
+    pub page_stride: i64,
+    pub token_stride: i64,
+    pub head_stride: i64,
+}
+
+/// wmi.h: one attention call over a paged cache (device pointers, strides in elements)
+#[repr(C)]
+#[derive(Debug, Copy, Clone)]
+pub struct wmi_paged_attn {
+    pub q: *const c_void,
+    pub out: *mut c_void,
+    pub block_table: *const c_int,
+    pub cu_q: *const c_int,
+    pub kv_lens: *const c_int,
+    pub q_row_stride: i64,
+    pub q_head_stride: i64,
+    pub out_row_stride: i64,
+    pub out_head_stride: i64,
+    pub table_stride: i64,
+    pub table_cols: c_int,
+    pub n_rows: c_int,
+    pub n_seq: c_int,
+    pub n_q_heads: c_int,
+    pub window: c_int,
+    pub max_new: c_int,
+    pub max_kv: c_int,
+    pub scale: c_float,
+}
+
 extern "C" {
     pub fn whisper_context_default_params() -> whisper_context_params;
     pub fn whisper_init_from_file_with_params(path_model: *const c_char, params: whisper_context_params) -> *mut whisper_context;
@@ -300,6 +345,19 @@ extern "C" {
     pub fn wmi_ingest_gate_plan(is_voice: *const u8, n_frames: i64, prefill: c_int, hangover: c_int, onset: c_int, src_out: *mut i64, cap: i64) -> i64;
     pub fn wmi_ingest_gather(frames_dev: *const c_float, n_frames: i64, src: *const i64, n_src: i64, out_dev: *mut c_float, out_cap: i64,
                              n_out: *mut i64, stream: *mut c_void) -> c_int;
+
+    // wmi.h: serving operators -- paged K/V cache and the draw of the next token (device pointers, enqueued on `stream`)
+    pub fn wmi_paged_plan(ctx_lens: *const c_int, new_lens: *const c_int, n_seq: c_int, free_pages: *const c_int, n_free: c_int, page_tokens: c_int,
+                          block_table: *mut c_int, table_cols: c_int, table_stride: i64, cu_q: *mut c_int, kv_lens: *mut c_int, slots: *mut c_int,
+                          positions: *mut c_int, n_rows_cap: c_int, counts: *mut c_int, stream: *mut c_void) -> c_int;
+    pub fn wmi_paged_write(cache: *const wmi_paged_cache, k_new: *const c_void, k_row_stride: i64, k_head_stride: i64, v_new: *const c_void,
+                           v_row_stride: i64, v_head_stride: i64, slots: *const c_int, n_rows: c_int, stream: *mut c_void) -> c_int;
+    pub fn wmi_paged_attention_workspace(cache: *const wmi_paged_cache, args: *const wmi_paged_attn) -> i64;
+    pub fn wmi_paged_attention(cache: *const wmi_paged_cache, args: *const wmi_paged_attn, workspace: *mut c_void, workspace_bytes: usize,
+                               stream: *mut c_void) -> c_int;
+    pub fn wmi_sample_tokens(logits: *const c_void, dtype: c_int, row_stride: i64, n_rows: c_int, n_vocab: c_int, uniform: *const c_float,
+                             temperature: *const c_float, top_k: *const c_int, top_p: *const c_float, min_p: *const c_float, token: *mut c_int,
+                             logprob: *mut c_float, stream: *mut c_void) -> c_int;
 }
 
 /// whisper-rs installs a ggml log hook through this symbol; the engine has no ggml, so it is a no-op
@@ -318,5 +376,7 @@ mod tests {
         assert_eq!(std::mem::size_of::<whisper_full_params>(), 264);
         assert_eq!(std::mem::size_of::<wmi_node_record>(), 40 + 4 * WMI_NODE_MAX_TOKENS);
         assert_eq!(std::mem::size_of::<wmi_kernel_stat>(), 24);
+        assert_eq!(std::mem::size_of::<wmi_paged_cache>(), 64);
+        assert_eq!(std::mem::size_of::<wmi_paged_attn>(), 112);
     }
 }

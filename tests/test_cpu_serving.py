@@ -1,0 +1,135 @@
+"""Refusals of the serving operators that need no GPU: the C entries check sizes, types, alignment and pointers before they touch the
+device, the Python layer checks shapes before it calls them. Plus the restatement's own sanity."""
+import ctypes as C
+import os
+import sys
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, ROOT)
+from handy_amd import serving as sv           # noqa: E402
+from handy_amd import whisper_rs as wr        # noqa: E402
+from oracle import serving_oracle as so       # noqa: E402
+
+
+class Fake:
+    """Something that looks like a device array and owns no memory (the entries must refuse before they would use it)."""
+
+    def __init__(self, shape, dtype, strides=None, ptr=0x10000):
+        self.shape, self.dtype, self._p = tuple(shape), dtype, ptr
+        self._s = tuple(strides) if strides is not None else sv._contiguous(self.shape)
+
+    def data_ptr(self): return self._p
+    def stride(self): return self._s
+    def numel(self): return int(np.prod(self.shape))
+
+
+P = 0x10000         # a non-null, aligned address that is no device memory
+
+
+def cache_struct(**kw):
+    c = dict(k=P, v=P, dtype=0, n_pages=8, page_tokens=16, n_kv_heads=2, head_dim=64, page_stride=2048, token_stride=128, head_stride=64)
+    c.update(kw)
+    return wr.wmi_paged_cache(*[c[n] for n, _ in wr.wmi_paged_cache._fields_])
+
+
+def attn_struct(**kw):
+    a = dict(q=P, out=P, block_table=P, cu_q=P, kv_lens=P, q_row_stride=256, q_head_stride=64, out_row_stride=256, out_head_stride=64, table_stride=8, table_cols=8,
+             n_rows=3, n_seq=3, n_q_heads=4, window=0, max_new=1, max_kv=100, scale=0.125)
+    a.update(kw)
+    return wr.wmi_paged_attn(*[a[n] for n, _ in wr.wmi_paged_attn._fields_])
+
+
+def test_attention_entry_refuses():
+    L = wr.load_library()
+    call = lambda c, a: L.wmi_paged_attention(C.byref(c), C.byref(a), None, 0, None)
+    for bad in (dict(k=None), dict(v=None), dict(dtype=2), dict(dtype=-1), dict(n_pages=0), dict(n_kv_heads=0), dict(head_dim=0), dict(page_stride=-8), dict(k=P + 2), dict(v=P + 8),
+                dict(token_stride=100), dict(head_stride=4)):
+        assert call(cache_struct(**bad), attn_struct()) == -1, bad
+    for bad in (dict(page_tokens=0), dict(page_tokens=12), dict(page_tokens=2048), dict(page_tokens=-16), dict(head_dim=60), dict(head_dim=136), dict(n_pages=2 ** 30)):
+        assert call(cache_struct(**bad), attn_struct()) == -3, bad
+    for bad in (dict(q=None), dict(out=None), dict(block_table=None), dict(cu_q=None), dict(kv_lens=None), dict(n_q_heads=3), dict(n_q_heads=0), dict(n_rows=-1), dict(n_seq=-1),
+                dict(table_cols=-1), dict(table_stride=7), dict(window=-1), dict(max_new=-1), dict(max_kv=-2), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=P + 4), dict(out=P + 2),
+                dict(q_row_stride=-256), dict(out_head_stride=-64), dict(q_head_stride=63), dict(out_row_stride=255)):
+        assert call(cache_struct(), attn_struct(**bad)) == -1, bad
+    assert call(cache_struct(n_kv_heads=1), attn_struct(n_q_heads=129)) == -3
+    assert L.wmi_paged_attention(None, C.byref(attn_struct()), None, 0, None) == -1
+    assert L.wmi_paged_attention(C.byref(cache_struct()), None, None, 0, None) == -1
+    assert call(cache_struct(), attn_struct(n_rows=0)) == 0 and call(cache_struct(), attn_struct(n_seq=0)) == 0      # nothing to do
+    assert L.wmi_paged_attention_workspace(C.byref(cache_struct(head_dim=60)), C.byref(attn_struct())) == -3
+    assert L.wmi_paged_attention_workspace(C.byref(cache_struct()), C.byref(attn_struct(q=None, out=None))) >= 0      # sizes only
+
+
+def test_plan_write_sample_entries_refuse():
+    L = wr.load_library()
+    def plan(**kw):
+        a = dict(ctx=P, new=P, n_seq=3, free=P, n_free=2, page=16, table=P, cols=4, stride=4, cu=P, kv=P, slots=P, pos=P, cap=5, counts=P)
+        a.update(kw)
+        return L.wmi_paged_plan(a["ctx"], a["new"], a["n_seq"], a["free"], a["n_free"], a["page"], a["table"], a["cols"], a["stride"], a["cu"], a["kv"], a["slots"], a["pos"], a["cap"],
+                                a["counts"], None)
+    for bad in (dict(ctx=None), dict(new=None), dict(free=None), dict(table=None), dict(cu=None), dict(kv=None), dict(slots=None), dict(pos=None), dict(counts=None), dict(n_seq=-1),
+                dict(n_free=-1), dict(cols=-1), dict(cap=-1), dict(stride=3)):
+        assert plan(**bad) == -1, bad
+    for bad in (dict(page=0), dict(page=24), dict(page=4096), dict(n_seq=16385), dict(cols=2 ** 27, stride=2 ** 27)):
+        assert plan(**bad) == -3, bad
+    write = lambda c, n=3, k=P, v=P, s=P, row=128: L.wmi_paged_write(C.byref(c), k, row, 64, v, row, 64, s, n, None)
+    assert write(cache_struct(), n=-1) == -1 and write(cache_struct(), k=None) == -1 and write(cache_struct(), v=None) == -1 and write(cache_struct(), s=None) == -1
+    assert write(cache_struct(), row=-128) == -1 and write(cache_struct(dtype=2)) == -1 and write(cache_struct(page_tokens=3)) == -3 and write(cache_struct(), n=0) == 0
+    def sample(**kw):
+        a = dict(x=P, dt=2, stride=50, rows=2, V=50, u=P, tok=P)
+        a.update(kw)
+        return L.wmi_sample_tokens(a["x"], a["dt"], a["stride"], a["rows"], a["V"], a["u"], None, None, None, None, a["tok"], None, None)
+    for bad in (dict(x=None), dict(u=None), dict(tok=None), dict(dt=3), dict(dt=-1), dict(rows=-1), dict(V=0), dict(stride=-1), dict(x=P + 2)):
+        assert sample(**bad) == -1, bad
+    assert sample(V=262145, stride=262145) == -3 and sample(rows=0) == 0
+
+
+def test_python_layer_refuses_wrong_shapes_and_types():
+    kv = lambda **kw: Fake(kw.get("shape", (8, 16, 2, 64)), kw.get("dtype", "float16"), kw.get("strides"))
+    cache = sv.PagedCache(kv(), kv())
+    for k, v in ((kv(dtype="float32"), kv(dtype="float32")), (kv(), kv(dtype="bfloat16")), (kv(), kv(shape=(8, 16, 2, 72))), (kv(shape=(8, 16, 128)), kv(shape=(8, 16, 128))),
+                 (kv(), kv(strides=(2048, 64, 1024, 1))), (kv(strides=(2048, 128, 1, 2)), kv(strides=(2048, 128, 1, 2)))):
+        with pytest.raises(ValueError):
+            sv.PagedCache(k, v)
+    i32 = lambda *s: Fake(s, "int32")
+    good = dict(q=Fake((5, 4, 64), "float16"), block_table=i32(3, 8), cu_q=i32(4), kv_lens=i32(3), out=Fake((5, 4, 64), "float16"))
+    for bad in (dict(q=Fake((5, 4, 72), "float16")), dict(q=Fake((5, 4, 64), "bfloat16")), dict(out=Fake((4, 4, 64), "float16")), dict(block_table=i32(2, 8)),
+                dict(block_table=Fake((3, 8), "int64")), dict(cu_q=i32(3)), dict(kv_lens=Fake((3,), "float32")), dict(out=Fake((5, 4, 64), "float16", (256, 1, 4))),
+                dict(q=Fake((5, 3, 64), "float16"), out=Fake((5, 3, 64), "float16"))):
+        a = {**good, **bad}
+        with pytest.raises(ValueError):
+            sv.paged_attention(a["q"], cache, a["block_table"], a["cu_q"], a["kv_lens"], 1, 100, a["out"])
+    with pytest.raises(ValueError):
+        sv.paged_attention(good["q"], cache, good["block_table"], good["cu_q"], good["kv_lens"], 1, 100, good["out"], workspace=Fake((64,), "float32"))
+    new = Fake((3, 2, 64), "float16")
+    for a in ((Fake((3, 2, 72), "float16"), new, i32(3)), (new, Fake((2, 2, 64), "float16"), i32(3)), (new, new, i32(2)), (new, new, Fake((3,), "int64")), (Fake((3, 2, 64), "bfloat16"), new, i32(3))):
+        with pytest.raises(ValueError):
+            sv.write_kv(cache, *a)
+    plan = sv.PagePlan(i32(4), i32(3), i32(9), i32(9), i32(4))
+    for a in ((i32(3), i32(2), i32(5), i32(3, 4), plan), (i32(3), i32(3), i32(5), i32(2, 4), plan), (i32(3), i32(3), Fake((5,), "int64"), i32(3, 4), plan),
+              (i32(3), i32(3), i32(5), i32(3, 4), plan._replace(cu_q=i32(3))), (i32(3), i32(3), i32(5), i32(3, 4), plan._replace(positions=i32(8)))):
+        with pytest.raises(ValueError):
+            sv.plan_pages(a[0], a[1], a[2], a[3], 16, a[4])
+    x, u, t = Fake((2, 50), "float32"), Fake((2,), "float32"), i32(2)
+    for a, kw in (((Fake((2, 50), "float64"), u, t), {}), ((Fake((100,), "float32"), u, t), {}), ((x, Fake((1,), "float32"), t), {}), ((x, u, Fake((2,), "int64")), {}),
+                  ((x, u, t), dict(top_k=Fake((2,), "float32"))), ((x, u, t), dict(temperature=i32(2))), ((x, u, t), dict(logprob=Fake((2,), "float16"))),
+                  ((Fake((2, 50), "float32", (1, 2)), u, t), {})):
+        with pytest.raises(ValueError):
+            sv.sample_tokens(*a, **kw)
+
+
+def test_restatement_on_cases_worked_by_hand():
+    t, cu, kv, slots, pos, counts = so.plan([3, 4], [2, 5], [9, 8, 7], 4, np.array([[1, -1, -1], [0, -1, -1]], np.int32), 8)
+    assert t.tolist() == [[1, 9, -1], [0, 8, 7]] and cu.tolist() == [0, 2, 7] and kv.tolist() == [5, 9]
+    assert slots.tolist() == [7, 36, 32, 33, 34, 35, 28, -1] and pos.tolist() == [3, 4, 4, 5, 6, 7, 8, 0] and counts.tolist() == [2, 7, 3, 0]
+    x = np.log(np.array([[0.1, 0.4, 0.2, 0.3]]))
+    at = lambda u, **kw: int(so.sample(x, np.array([u], np.float32), **kw)[0][0])
+    assert [at(u) for u in (0.0, 0.09, 0.11, 0.49, 0.51, 0.69, 0.71, 0.999)] == [0, 0, 1, 1, 2, 2, 3, 3]
+    assert [at(u, top_k=[2]) for u in (0.0, 0.57, 0.58)] == [1, 1, 3]                 # 0.4 and 0.3 in the vocabulary's order: border 4/7
+    assert [at(u, top_p=[0.75]) for u in (0.4, 0.5, 0.7)] == [1, 2, 3]                # 0.4 + 0.3 < 0.75: three are kept
+    assert at(0.99, min_p=[0.6]) == 3 and at(0.99, min_p=[0.8]) == 1 and at(0.3, temperature=[0.0]) == 1
+    k = np.zeros((1, 4, 1, 2)); v = np.arange(8.0).reshape(1, 4, 1, 2)
+    out, _, _ = so.attention(np.zeros((2, 1, 2)), k, v, np.array([[0]]), [0, 2], [3], 4, 1.0)
+    assert out[:, 0].tolist() == [[1.0, 2.0], [2.0, 3.0]]                             # means of the first two and three values
