@@ -2,6 +2,7 @@
 // V into their slots, and attention of a chunk of new tokens (or one token) over the cache.
 #include "kernels.h"
 #include "serving_host.h"
+#include <type_traits>
 
 namespace wmi {
 
@@ -122,97 +123,602 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------ attention
-// One workgroup per (row, query head): 8 or 16 lanes share a key (8 dims each), every lane group keeps its own running maximum,
-// sum and accumulator over the keys it visits, and the groups are merged at the end.
-template <class T> struct Vec8;
-template <> struct Vec8<f16> { typedef f16x8 type; };
+// softmax(scale q K^T) V with the running maximum and sum of an online softmax. Both kernels compute, on MFMA,
+//   S^T = K Q^T     K rows as the A operand, so that a lane holds scores of ONE query row (its column)
+//   O^T += V^T P^T  P^T goes from the score registers straight into the B operand; V^T is read out of the row-major V tile with the
+//                   LDS transpose load (4 keys of one dim a lane), in the key order the score registers hold
+// The query rows of a request's tokens and of the heads that share a key head are packed into one list, row r = token * group +
+// head, so that every K and V byte is read once for all of them.
+//   paged_step_kernel    up to 16 packed rows (single tokens): bound by HBM. Each wave streams its own 16-key tiles.
+//   paged_chunk_kernel   128 packed rows a workgroup, 64-key tiles shared by its waves: bound by MFMA issue and LDS reads.
+// The keys of a tile of rows may be split over workgroups; paged_join_kernel adds the parts up.
+// The reference exponent of a row moves only when a score passes it by more than 8 (in powers of two): probabilities stay below
+// 2^8, which both 16-bit types hold at full relative precision, and the accumulators are rescaled rarely instead of every tile.
 typedef __bf16 bf16;
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
-template <> struct Vec8<bf16> { typedef bf16x8 type; };
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-template <class T, int LPK>       // LPK lanes a key
-__global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
-    typedef typename Vec8<T>::type V8;
-    constexpr int KPW = 64 / LPK;
-    __shared__ float red[4][LPK][10];
-    const int row = blockIdx.x, hq = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, grp = lane / LPK, e = (lane % LPK) * 8;
-    int lo = 0, hi = a.n_seq;                                 // the request of this row
-    while (lo < hi) { const int m = (lo + hi) >> 1; if (a.cu[m + 1] <= row) lo = m + 1; else hi = m; }
-    if (lo >= a.n_seq || row < a.cu[lo]) return;              // rows behind the last request stay as they are
-    const int i = lo, n = a.cu[i + 1] - a.cu[i];
-    const int L = min(max(a.kv_lens[i], 0), (int)min((long)a.cols << a.lp, 0x7fffffffL));
-    const int pos = L - n + (row - a.cu[i]);
-    const int k0 = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    const int h = hq / a.group;
-    const bool on = e < a.dim;
-    const T *kc = (const T *)a.k + h * a.head_stride + e, *vc = (const T *)a.v + h * a.head_stride + e;
-    float q[8], acc[8], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int t = 0; t < 8; t++) { q[t] = 0.0f; acc[t] = 0.0f; }
-    if (on) { const V8 x = *(const V8 *)((const T *)a.q + row * a.q_row + hq * a.q_head + e);
-#pragma unroll
-        for (int t = 0; t < 8; t++) q[t] = (float)x[t] * a.scale; }
-    for (int j = k0 + wave * KPW + grp; j <= pos; j += 4 * KPW) {
-        const int page = a.table[i * a.table_stride + (j >> a.lp)];
-        if (page < 0 || page >= a.n_pages) continue;
-        const long off = page * a.page_stride + (long)(j & ((1 << a.lp) - 1)) * a.token_stride;
-        float d = 0.0f;
-        V8 vx = {};
-        if (on) {
-            const V8 kx = *(const V8 *)(kc + off);
-            vx = *(const V8 *)(vc + off);
-#pragma unroll
-            for (int t = 0; t < 8; t++) d = __builtin_fmaf(q[t], (float)kx[t], d);
-        }
-#pragma unroll
-        for (int o = 1; o < LPK; o <<= 1) d += __shfl_xor(d, o);
-        const float mn = fmaxf(m, d), al = m == -INFINITY ? 0.0f : __expf(m - mn), p = __expf(d - mn);
-        l = l * al + p;
-#pragma unroll
-        for (int t = 0; t < 8; t++) acc[t] = acc[t] * al + p * (float)vx[t];
-        m = mn;
+template <class T> struct Mma;
+template <> struct Mma<f16> {
+    typedef f16x8 V8; typedef f16x4 V4;
+    static constexpr unsigned short kExp = 0x7c00, kOne = 0x3c00, kSign = 0x8000;
+    static __device__ __forceinline__ f32x16 m32(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 m16k32(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 m16k16(V4 a, V4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma<bf16> {
+    typedef bf16x8 V8; typedef bf16x4 V4;
+    static constexpr unsigned short kExp = 0x7f80, kOne = 0x3f80, kSign = 0x8000;
+    static __device__ __forceinline__ f32x16 m32(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 m16k32(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 m16k16(V4 a, V4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
     }
-    for (int o = LPK; o < 64; o <<= 1) {
-        const float om = __shfl_xor(m, o), ol = __shfl_xor(l, o), mn = fmaxf(m, om);
-        const float fa = m == -INFINITY ? 0.0f : __expf(m - mn), fb = om == -INFINITY ? 0.0f : __expf(om - mn);
-        l = l * fa + ol * fb;
+};
+
+#define WMI_LDS __attribute__((address_space(3)))
+#define WMI_GLB __attribute__((address_space(1)))
+
+// LDS transpose loads: 16 lanes hand in the addresses of 4 rows x 16 columns (lane i: row i / 4, columns 4 (i % 4) ..), each gets one
+// column's 4 rows. N of them at LDS addresses ad[] + OFF, waited for in the same block: as a builtin the compiler would also wait
+// for every LDS-DMA in flight before each of them, the next tile's included.
+__device__ __forceinline__ unsigned lds_addr(const char *p) { return (unsigned)(uintptr_t)(const WMI_LDS char *)p; }
+template <int OFF> __device__ __forceinline__ void lds_read_tr(const unsigned (&ad)[4], s16x4 (&v)[4]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%8\n\tds_read_b64_tr_b16 %1, %5 offset:%8\n\tds_read_b64_tr_b16 %2, %6 offset:%8\n\t"
+                 "ds_read_b64_tr_b16 %3, %7 offset:%8\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(ad[0]), "v"(ad[1]), "v"(ad[2]), "v"(ad[3]), "n"(OFF) : "memory");
+}
+template <int OFF> __device__ __forceinline__ void lds_read_tr(const unsigned (&ad)[8], s16x4 (&v)[8]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %9 offset:%16\n\tds_read_b64_tr_b16 %2, %10 offset:%16\n\t"
+                 "ds_read_b64_tr_b16 %3, %11 offset:%16\n\tds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
+                 "ds_read_b64_tr_b16 %6, %14 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%16\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+                 : "v"(ad[0]), "v"(ad[1]), "v"(ad[2]), "v"(ad[3]), "v"(ad[4]), "v"(ad[5]), "v"(ad[6]), "v"(ad[7]), "n"(OFF) : "memory");
+}
+
+// K and V tiles lie in the LDS as rows of DP elements, their 16-byte chunks permuted by row (chunk ^ swz(row)): the chunks that one
+// fragment read touches (one chunk of 16 rows, or four chunks of four rows) then fall into different banks.
+template <int DP> __device__ __forceinline__ int swz(int row) { return DP == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3); }
+
+__device__ __attribute__((aligned(16))) unsigned attn_zero_chunk[4];     // what lanes without a key load
+
+struct AttnReq { int q0, n, len; };
+// lengths and offsets of a request, forced into the call's buffers whatever the arrays hold
+__device__ __forceinline__ AttnReq attn_req(const PagedAttn &a, int i) {
+    AttnReq r;
+    r.q0 = min(max(a.cu[i], 0), a.n_rows);
+    r.n = min(max(a.cu[i + 1], r.q0), a.n_rows) - r.q0;
+    const long room = (long)a.cols << a.lp;
+    r.len = (int)min((long)max(a.kv_lens[i], 0), min(room, 0x7fffffffL));
+    return r;
+}
+// keys [lo, hi) that the packed rows r0 .. r1 - 1 of a request see between them
+__device__ __forceinline__ void attn_keys(const PagedAttn &a, const AttnReq &q, int r0, int r1, int &lo, int &hi) {
+    const int first = q.len - q.n + r0 / a.group, last = q.len - q.n + (r1 - 1) / a.group;
+    hi = max(last + 1, 0);
+    lo = a.window > 0 ? max(first - a.window + 1, 0) : 0;
+}
+// how many parts the keys of a tile of rows are cut into: at most `splits`, none shorter than `least` key tiles
+__device__ __forceinline__ int attn_parts(int n_kt, int splits, int least) { return max(1, min(splits, n_kt / least)); }
+
+constexpr int kStepRows = 16, kStepKeys = 16, kChunkRows = 128, kChunkKeys = 64;
+constexpr int kStepLeast = 32, kChunkLeast = 4;        // shortest part, in key tiles (512 and 256 keys): below that the join costs more than it saves
+constexpr float kMoveBy = 8.0f;
+
+// partial results of a split call: [part][row][query head][DP] accumulators, then {reference exponent, sum}
+struct AttnParts { float *o; float2 *ml; int splits; };
+
+template <class T> __device__ __forceinline__ u16x4 not_finite(typename Mma<T>::V4 v) {
+    const u16x4 b = __builtin_bit_cast(u16x4, v);
+    return (u16x4)((b & Mma<T>::kExp) == Mma<T>::kExp);                    // all ones where infinite or NaN
+}
+template <class T> __device__ __forceinline__ u16x8 not_finite8(typename Mma<T>::V8 v) {
+    const u16x8 b = __builtin_bit_cast(u16x8, v);
+    return (u16x8)((b & Mma<T>::kExp) == Mma<T>::kExp);
+}
+__device__ __forceinline__ bool any_set(u16x4 v) { const uint2 w = __builtin_bit_cast(uint2, v); return (w.x | w.y) != 0; }
+__device__ __forceinline__ bool any_set(u16x8 v) { const uint4 w = __builtin_bit_cast(uint4, v); return (w.x | w.y | w.z | w.w) != 0; }
+
+// ---- single tokens (and any rows at all, 16 at a time)
+// One workgroup = (request, key head, part of the keys); its 4 waves take 16-key tiles in turn, each through two LDS buffers of its
+// own filled by LDS-DMA (no barrier in the loop: a wave waits for its own loads only, counted, so that the next tile is always on
+// its way). A tile's page is one table entry (PAGE16: pages of 16 tokens and more); 64 tiles' entries are read at a time.
+template <class T, int DP, bool PAGE16>
+__global__ __launch_bounds__(256, 2) void paged_step_kernel(PagedAttn a, AttnParts ps) {
+    typedef Mma<T> M;
+    typedef typename M::V8 V8;
+    typedef typename M::V4 V4;
+    constexpr int CH = DP / 8, RPI = 64 / CH, NI = kStepKeys / RPI, TILE = kStepKeys * DP * 2, NB = DP / 16, NK = DP / 32;
+    __shared__ __attribute__((aligned(16))) char smem[4 * 2 * 2 * TILE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g4 = lane >> 4;
+    const int head = blockIdx.x % a.hkv, req = blockIdx.x / a.hkv, part = blockIdx.y;
+    const AttnReq rq = attn_req(a, req);
+    const int rows = rq.n * a.group, *tbl = a.table + req * a.table_stride;
+    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-38f);    // a negative scale turns q round; 0 leaves equal scores
+    const T *kc = (const T *)a.k + head * a.head_stride, *vc = (const T *)a.v + head * a.head_stride;
+    char *mine = smem + wave * 4 * TILE;
+    const int lrow = lane / CH, lslot = lane % CH;
+
+    for (int r0 = 0; r0 < rows; r0 += kStepRows) {
+        const int r1 = min(rows, r0 + kStepRows);
+        int lo, hi;
+        attn_keys(a, rq, r0, r1, lo, hi);
+        const int kt0 = lo / kStepKeys, n_kt = max((hi + kStepKeys - 1) / kStepKeys - kt0, 0), parts = attn_parts(n_kt, ps.splits, kStepLeast);
+        if (part >= parts) continue;
+        const int t0 = kt0 + (int)((long)n_kt * part / parts) + wave, t1 = kt0 + (int)((long)n_kt * (part + 1) / parts);
+        const int row = min(r0 + n16, r1 - 1), tok = row / a.group, hq = head * a.group + row % a.group, pos = rq.len - rq.n + tok;
+        const int first = rq.len - rq.n + r0 / a.group, klow = a.window > 0 ? pos - a.window + 1 : 0;
+        const bool one = r0 / a.group == (r1 - 1) / a.group;               // one token: every key in [lo, hi) is seen by every row
+        V8 qf[NK];
 #pragma unroll
-        for (int t = 0; t < 8; t++) { const float oa = __shfl_xor(acc[t], o); acc[t] = acc[t] * fa + oa * fb; }
-        m = mn;
-    }
-    if (grp == 0) { red[wave][lane][0] = m; red[wave][lane][1] = l;
-#pragma unroll
-        for (int t = 0; t < 8; t++) red[wave][lane][2 + t] = acc[t]; }
-    __syncthreads();
-    if (tid < LPK && on) {
-        float mn = -INFINITY, ls = 0.0f, o[8] = {};
-        for (int w = 0; w < 4; w++) mn = fmaxf(mn, red[w][tid][0]);
-        for (int w = 0; w < 4; w++) {
-            const float f = red[w][tid][0] == -INFINITY ? 0.0f : __expf(red[w][tid][0] - mn);
-            ls += red[w][tid][1] * f;
-#pragma unroll
-            for (int t = 0; t < 8; t++) o[t] += red[w][tid][2 + t] * f;
+        for (int ks = 0; ks < NK; ks++) {
+            u16x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
+            const int e = ks * 32 + g4 * 8;
+            if (e < a.dim) x = *(const u16x8 *)((const T *)a.q + (rq.q0 + tok) * a.q_row + hq * a.q_head + e);
+            if (a.scale < 0.0f) x ^= M::kSign;
+            qf[ks] = __builtin_bit_cast(V8, x);
         }
-        const float inv = ls > 0.0f ? 1.0f / ls : 0.0f;      // a row that sees nothing gives zeros
-        V8 y;
+        f32x4 o[NB];
 #pragma unroll
-        for (int t = 0; t < 8; t++) y[t] = (T)(o[t] * inv);
-        *(V8 *)((T *)a.out + row * a.o_row + hq * a.o_head + e) = y;
+        for (int i = 0; i < NB; i++) o[i] = f32x4{0, 0, 0, 0};
+        float m = -INFINITY, l = 0.0f;
+        int pg[PAGE16 ? 1 : NI];
+        // table entries: PAGE16 -- lane x holds the entry of this wave's tile number (base + x); else one entry per load and lane
+        auto entries = [&](int t) {
+            if constexpr (PAGE16) {
+                const long j = (long)(t + 4 * lane) * kStepKeys;
+                pg[0] = j < hi ? tbl[j >> a.lp] : -1;
+                __builtin_amdgcn_s_waitcnt(0xf70);                         // vmcnt(0): once in 64 tiles, so that the loop's waits stay counted
+            } else {
+#pragma unroll
+                for (int i = 0; i < NI; i++) {                             // always loaded (clamped into the keys): the loop counts on NI loads
+                    const int j = t * kStepKeys + i * RPI + lrow, e = tbl[min(max(j, lo), hi - 1) >> a.lp];
+                    pg[i] = j >= lo && j < hi ? e : -1;
+                }
+            }
+        };
+        auto page_ok = [&](int p) { return (unsigned)p < (unsigned)a.n_pages; };
+        auto stage = [&](int t, int buf, int at) {
+            char *kd = mine + buf * 2 * TILE;
+            const int up = PAGE16 ? __builtin_amdgcn_readlane(pg[0], at) : 0;
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int lr = i * RPI + lrow, j = t * kStepKeys + lr, ch = lslot ^ swz<DP>(lr), page = PAGE16 ? up : pg[i];
+                const bool on = j >= lo && j < hi && page_ok(page) && ch * 8 < a.dim;
+                const long off = page * a.page_stride + (long)(j & ((1 << a.lp) - 1)) * a.token_stride + ch * 8;
+                const T *ksrc = on ? kc + off : (const T *)attn_zero_chunk, *vsrc = on ? vc + off : (const T *)attn_zero_chunk;
+                __builtin_amdgcn_global_load_lds((const WMI_GLB void *)ksrc, (WMI_LDS void *)(kd + i * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const WMI_GLB void *)vsrc, (WMI_LDS void *)(kd + TILE + i * 1024), 16, 0, 0);
+            }
+        };
+        auto compute = [&](int t, int buf, bool page_bad, unsigned bad_keys) {
+            const char *kb = mine + buf * 2 * TILE, *vb = kb + TILE;
+            f32x4 s = {0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < NK; ks++) s = M::m16k32(*(const V8 *)(kb + n16 * DP * 2 + (((ks * 4 + g4) ^ swz<DP>(n16)) << 4)), qf[ks], s);
+            const int k0 = t * kStepKeys;
+            const bool cut = k0 < lo || k0 + kStepKeys > hi || page_bad, mixed = !one && (k0 + kStepKeys - 1 > first || a.window > 0);
+            if (cut || mixed) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int kk = g4 * 4 + r, j = k0 + kk;
+                    if (j > pos || j < klow || j < lo || j >= hi || ((bad_keys >> kk) & 1)) s[r] = -INFINITY;
+                }
+            }
+            const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) * c;
+            if (__any(mx > m + kMoveBy)) {
+                float mn = fmaxf(mx, __shfl_xor(mx, 16));
+                mn = fmaxf(fmaxf(mn, __shfl_xor(mn, 32)), m);
+                const float al = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+                l *= al;
+#pragma unroll
+                for (int i = 0; i < NB; i++) o[i] *= al;
+                m = mn;
+            }
+            const float mu = m == -INFINITY ? 0.0f : m;
+            V4 p;
+#pragma unroll
+            for (int r = 0; r < 4; r++) { const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -mu)); l += e; p[r] = (T)e; }
+            unsigned ad[NB];
+            s16x4 raw[NB];
+            V4 v[NB];
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                const int kr = g4 * 4 + (n16 >> 2), ch = i * 2 + ((n16 & 3) >> 1);
+                ad[i] = lds_addr(vb + kr * DP * 2 + ((ch ^ swz<DP>(kr)) << 4) + (n16 & 1) * 8);
+            }
+            lds_read_tr<0>(ad, raw);
+#pragma unroll
+            for (int i = 0; i < NB; i++) v[i] = __builtin_bit_cast(V4, raw[i]);
+            if (mixed) {                                                   // keys that some rows see and others do not: see seen_only below
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < NB; i++) bad |= any_set(not_finite<T>(v[i]));
+                if (__any(bad)) {
+                    u16x4 see;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) see[r] = s[r] == -INFINITY ? 0 : M::kOne;
+#pragma unroll
+                    for (int i = 0; i < NB; i++) {
+                        const u16x4 nf = not_finite<T>(v[i]);
+                        const f32x4 cnt = M::m16k16(__builtin_bit_cast(V4, (u16x4)(nf & M::kOne)), __builtin_bit_cast(V4, see), f32x4{0, 0, 0, 0});
+                        v[i] = __builtin_bit_cast(V4, (u16x4)(__builtin_bit_cast(u16x4, v[i]) & ~nf));
+#pragma unroll
+                        for (int r = 0; r < 4; r++) if (cnt[r] > 0.0f) o[i][r] = NAN;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NB; i++) o[i] = M::m16k16(v[i], p, o[i]);
+        };
+        if (t0 < t1) {
+            // bit kk: key kk of the tile lies on a page the cache does not have
+            auto bad_of = [&](int at) -> unsigned {
+                if constexpr (PAGE16) return page_ok(__builtin_amdgcn_readlane(pg[0], at)) ? 0u : 0xffffu;
+                else {
+                    unsigned b = 0;
+#pragma unroll
+                    for (int i = 0; i < NI; i++) {
+                        const unsigned long long v = __ballot(!page_ok(pg[i]));
+#pragma unroll
+                        for (int r = 0; r < RPI; r++) b |= (unsigned)((v >> (r * CH)) & 1) << (i * RPI + r);
+                    }
+                    return b;
+                }
+            };
+            entries(t0);
+            unsigned bad_now = bad_of(0), bad_next = 0;
+            stage(t0, 0, 0);
+            if constexpr (!PAGE16) entries(t0 + 4);
+            int k = 1, buf = 0;                                            // k: number of the next tile within the 64 whose entries are held
+            for (int t = t0; t < t1; t += 4, buf ^= 1) {
+                const int tn = t + 4;
+                if (tn < t1) {
+                    if constexpr (PAGE16) { if (k == 64) { entries(tn); k = 0; } }
+                    bad_next = bad_of(k);
+                    stage(tn, buf ^ 1, k);
+                    if constexpr (!PAGE16) entries(tn + 4);
+                    k++;
+                    if constexpr (PAGE16) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
+                    else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NI) : "memory");
+                } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                compute(t, buf, bad_now != 0, bad_now);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // this buffer's reads are done before the next loads into it go out
+                bad_now = bad_next;
+            }
+        }
+        // the four waves' parts meet in the LDS
+        l += __shfl_xor(l, 16); l += __shfl_xor(l, 32);
+        __syncthreads();
+        float *red = (float *)smem;                                        // [wave][row][DP + 2]
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) red[(wave * kStepRows + n16) * (DP + 2) + i * 16 + g4 * 4 + r] = o[i][r];
+        if (g4 == 0) { red[(wave * kStepRows + n16) * (DP + 2) + DP] = m; red[(wave * kStepRows + n16) * (DP + 2) + DP + 1] = l; }
+        __syncthreads();
+        for (int x = tid; x < (r1 - r0) * (DP / 4); x += 256) {
+            const int rr = x / (DP / 4), e = (x % (DP / 4)) * 4;
+            if (e >= a.dim) continue;
+            const float *w0 = red + rr * (DP + 2);
+            constexpr int WS = kStepRows * (DP + 2);
+            float mm = -INFINITY, ll = 0.0f, acc[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < 4; w++) mm = fmaxf(mm, w0[w * WS + DP]);
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float mw = w0[w * WS + DP], f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - mm);
+                ll += w0[w * WS + DP + 1] * f;
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[r] += w0[w * WS + e + r] * f;
+            }
+            const int pr = r0 + rr, orow = rq.q0 + pr / a.group, oh = head * a.group + pr % a.group;
+            if (parts == 1) {
+                const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;           // a row that sees nothing gives zeros
+                V4 y;
+#pragma unroll
+                for (int r = 0; r < 4; r++) y[r] = (T)(acc[r] * inv);
+                *(V4 *)((T *)a.out + orow * a.o_row + oh * a.o_head + e) = y;
+            } else {
+                const long at = ((long)part * a.n_rows + orow) * (a.hkv * a.group) + oh;
+                *(f32x4 *)(ps.o + at * DP + e) = f32x4{acc[0], acc[1], acc[2], acc[3]};
+                if (e == 0) ps.ml[at] = make_float2(mm, ll);
+            }
+        }
+        __syncthreads();
     }
 }
 
-size_t paged_attention_workspace(const PagedAttn &) { return 0; }
+// ---- chunks of new tokens
+// One workgroup = 128 packed rows of a request (32 a wave), one key head, one part of the keys. A row tile is found from the
+// workgroup's number alone: request i's tiles start at number floor(cu[i] * group / 128) + i, which leaves room for all of them
+// (a few numbers stay empty). Workgroups are dealt round-robin to the 8 XCDs: every XCD gets a contiguous run of (head, row
+// tile), so that the row tiles that stream the same keys share an L2, the ones with the most keys first.
+// Keys a row sees and others of its tile do not are masked to -infinity, p = 0; what V holds there must not be infinite or NaN in
+// the product, so in tiles that need a mask such values are taken out and reach only the rows that do see them (as NaN).
+template <class T, int DP>
+__global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a, AttnParts ps, int n_tiles) {
+    typedef Mma<T> M;
+    typedef typename M::V8 V8;
+    typedef typename M::V4 V4;
+    constexpr int CH = DP / 8, RPI = 64 / CH, NI = kChunkKeys / RPI / 4, TILE = kChunkKeys * DP * 2, NB = DP / 32, NK = DP / 16;
+    __shared__ __attribute__((aligned(16))) char smem[2 * 2 * TILE];
+    __shared__ __attribute__((aligned(16))) unsigned bad_flag[2][4];       // per buffer: some key of this wave's share has no page ...
+    __shared__ unsigned char bad_key[2][kChunkKeys];                       // ... and which
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n32 = lane & 31, h = lane >> 5;
+    const int nblk = gridDim.x, xq = nblk >> 3, xr = nblk & 7, xcd = blockIdx.x & 7, xi = blockIdx.x >> 3;
+    const int logical = (xcd < xr ? xcd * (xq + 1) : xr * (xq + 1) + (xcd - xr) * xq) + xi;
+    const int part = logical % ps.splits, tile = n_tiles - 1 - (logical / ps.splits) % n_tiles, head = logical / ps.splits / n_tiles;
+    int req = 0;
+    for (int left = a.n_seq; left > 1;) {                                  // the last request whose first tile number is <= tile, 64 ways at a time
+        const int step = (left + 63) / 64, i = req + lane * step;
+        const bool ok = lane * step < left && (long)a.cu[i] * a.group / kChunkRows + i <= tile;
+        const int k = max(__popcll(__ballot(ok)) - 1, 0);
+        req += k * step; left = min(step, left - k * step);
+    }
+    req = __builtin_amdgcn_readfirstlane(req);
+    const AttnReq rq = attn_req(a, req);
+    const long r0l = ((long)tile - ((long)a.cu[req] * a.group / kChunkRows + req)) * kChunkRows;
+    const int rows = rq.n * a.group;
+    if (r0l < 0 || r0l >= rows) return;
+    const int r0 = (int)r0l, r1 = min(rows, r0 + kChunkRows);
+    int lo, hi;
+    attn_keys(a, rq, r0, r1, lo, hi);
+    const int kt0 = lo / kChunkKeys, n_kt = max((hi + kChunkKeys - 1) / kChunkKeys - kt0, 0), parts = attn_parts(n_kt, ps.splits, kChunkLeast);
+    if (part >= parts) return;
+    const int t0 = kt0 + (int)((long)n_kt * part / parts), t1 = kt0 + (int)((long)n_kt * (part + 1) / parts);
+    const int *tbl = a.table + req * a.table_stride;
+    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-38f);
+    const T *kc = (const T *)a.k + head * a.head_stride, *vc = (const T *)a.v + head * a.head_stride;
 
-bool paged_attention(const PagedAttn &a, void *, hipStream_t st) {
-    const dim3 grid(a.n_rows, a.hkv * a.group);
-    if (a.dtype == WMI_F16) {
-        if (a.dim <= 64) hipLaunchKernelGGL((paged_attention_kernel<f16, 8>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((paged_attention_kernel<f16, 16>), grid, dim3(256), 0, st, a);
+    const int w0 = r0 + wave * 32, row = min(w0 + n32, r1 - 1), tok = row / a.group, hq = head * a.group + row % a.group, pos = rq.len - rq.n + tok;
+    const bool busy = w0 < r1;
+    const int pmin = rq.len - rq.n + w0 / a.group, pmax = rq.len - rq.n + (min(w0 + 32, r1) - 1) / a.group;   // this wave's positions
+    const int klow = a.window > 0 ? pos - a.window + 1 : 0;
+    V8 qf[NK];
+#pragma unroll
+    for (int ks = 0; ks < NK; ks++) {
+        u16x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
+        const int e = ks * 16 + h * 8;
+        if (e < a.dim) x = *(const u16x8 *)((const T *)a.q + (rq.q0 + tok) * a.q_row + hq * a.q_head + e);
+        if (a.scale < 0.0f) x ^= M::kSign;
+        qf[ks] = __builtin_bit_cast(V8, x);
+    }
+    const int lrow = lane / CH, lslot = lane % CH;
+    int pg[NI];
+    auto entries = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < NI; i++) { const int j = t * kChunkKeys + (wave + 4 * i) * RPI + lrow; pg[i] = j >= lo && j < hi ? tbl[j >> a.lp] : 0; }
+    };
+    auto stage = [&](int t, int buf) {
+        char *kd = smem + buf * 2 * TILE;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int lr = (wave + 4 * i) * RPI + lrow, j = t * kChunkKeys + lr, ch = lslot ^ swz<DP>(lr);
+            const bool has = (unsigned)pg[i] < (unsigned)a.n_pages, on = j >= lo && j < hi && has && ch * 8 < a.dim;
+            bad |= !has;
+            const long off = pg[i] * a.page_stride + (long)(j & ((1 << a.lp) - 1)) * a.token_stride + ch * 8;
+            const T *ksrc = on ? kc + off : (const T *)attn_zero_chunk, *vsrc = on ? vc + off : (const T *)attn_zero_chunk;
+            char *dst = kd + (wave + 4 * i) * 1024;
+            __builtin_amdgcn_global_load_lds((const WMI_GLB void *)ksrc, (WMI_LDS void *)dst, 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((const WMI_GLB void *)vsrc, (WMI_LDS void *)(dst + TILE), 16, 0, 0);
+        }
+        const bool any = __any(bad);
+        if (lane == 0) bad_flag[buf][wave] = any;
+        if (any && lslot == 0) {
+#pragma unroll
+            for (int i = 0; i < NI; i++) bad_key[buf][(wave + 4 * i) * RPI + lrow] = (unsigned)pg[i] >= (unsigned)a.n_pages;
+        }
+    };
+    f32x16 o[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[b][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    const int kf = n32 * DP * 2 + ((h ^ swz<DP>(n32)) << 4);               // K fragment ks of half kh: kb + kh * 32 rows + (kf ^ ks * 32)
+    const int vrow = 4 * h + ((lane & 15) >> 2), vcol = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    const int vf = vrow * DP * 2 + ((vcol ^ swz<DP>(vrow)) << 4) + (lane & 1) * 8;   // V^T of keys 8 x + vrow: vb + 8 x rows + (vf ^ block * 64 ^ (x & 1) * 32)
+    // V^T fragments of keys 16 s + {4 h + 0..3, 8 + 4 h + 0..3} for all blocks of 32 dims
+    auto read_v = [&](const unsigned (&ad)[2 * NB], auto s_tag, V8 (&v)[NB]) __attribute__((always_inline)) {
+        constexpr int S = decltype(s_tag)::value;
+        s16x4 raw[2 * NB];
+        lds_read_tr<16 * S * DP * 2>(ad, raw);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const s16x4 x = raw[2 * b], y = raw[2 * b + 1];
+            v[b] = __builtin_bit_cast(V8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    };
+
+    if (t0 < t1) { entries(t0); stage(t0, 0); entries(t0 + 1); }
+    for (int t = t0; t < t1; t++) {
+        const int buf = (t - t0) & 1, k0 = t * kChunkKeys;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // everybody's share of this tile has landed, the other buffer is free
+        if (t + 1 < t1) { stage(t + 1, buf ^ 1); entries(t + 2); }
+        if (!busy || k0 > pmax || (a.window > 0 && k0 + kChunkKeys <= pmin - a.window + 1)) continue;
+        const char *kb = smem + buf * 2 * TILE, *vb = kb + TILE;
+        f32x16 s[2];
+#pragma unroll
+        for (int kh = 0; kh < 2; kh++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[kh][i] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < NK; ks++) s[kh] = M::m32(*(const V8 *)(kb + kh * 32 * DP * 2 + (kf ^ (ks * 32))), qf[ks], s[kh]);
+        }
+        const uint4 fl = *(const uint4 *)bad_flag[buf];
+        const bool hole = __builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w) != 0;
+        const bool mixed = k0 + kChunkKeys - 1 > pmin || (a.window > 0 && k0 < pmax - a.window + 1) || hole;
+        if (mixed) {
+#pragma unroll
+            for (int kh = 0; kh < 2; kh++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int kk = kh * 32 + (i & 3) + 8 * (i >> 2) + 4 * h, j = k0 + kk;
+                    if (j > pos || j < klow) s[kh][i] = -INFINITY;
+                    if (hole && bad_flag[buf][(kk / RPI) & 3] && bad_key[buf][kk]) s[kh][i] = -INFINITY;
+                }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kh = 0; kh < 2; kh++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[kh][i]);
+        mx *= c;
+        if (__any(mx > m + kMoveBy)) {
+            const float mn = fmaxf(fmaxf(mx, __shfl_xor(mx, 32)), m), al = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= al;
+#pragma unroll
+            for (int b = 0; b < NB; b++) o[b] *= al;
+            m = mn;
+        }
+        const float mu = m == -INFINITY ? 0.0f : m;
+        V8 p[4];
+#pragma unroll
+        for (int kh = 0; kh < 2; kh++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kh][i], c, -mu));
+                l += e;
+                p[kh * 2 + (i >> 3)][i & 7] = (T)e;
+            }
+        unsigned ad[2 * NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) { ad[2 * b] = lds_addr(vb + (vf ^ (b * 64))); ad[2 * b + 1] = lds_addr(vb + 8 * DP * 2 + (vf ^ (b * 64) ^ 32)); }
+        auto pv = [&](auto x_tag) __attribute__((always_inline)) {
+            constexpr int X = decltype(x_tag)::value;
+            V8 v[NB];
+            read_v(ad, x_tag, v);
+            if (mixed) {
+                u16x8 bad = not_finite8<T>(v[0]);
+#pragma unroll
+                for (int b = 1; b < NB; b++) bad |= not_finite8<T>(v[b]);
+                if (__any(any_set(bad))) {
+                    u16x8 see;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) see[i] = s[X >> 1][(X & 1) * 8 + i] == -INFINITY ? 0 : M::kOne;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const u16x8 nf = not_finite8<T>(v[b]);
+                        f32x16 cnt;
+#pragma unroll
+                        for (int i = 0; i < 16; i++) cnt[i] = 0.0f;
+                        cnt = M::m32(__builtin_bit_cast(V8, (u16x8)(nf & M::kOne)), __builtin_bit_cast(V8, see), cnt);
+#pragma unroll
+                        for (int i = 0; i < 16; i++) if (cnt[i] > 0.0f) o[b][i] = NAN;
+                        v[b] = __builtin_bit_cast(V8, (u16x8)(__builtin_bit_cast(u16x8, v[b]) & ~nf));
+                    }
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++) o[b] = M::m32(v[b], p[X], o[b]);
+        };
+        pv(std::integral_constant<int, 0>());
+        pv(std::integral_constant<int, 1>());
+        pv(std::integral_constant<int, 2>());
+        pv(std::integral_constant<int, 3>());
+    }
+    l += __shfl_xor(l, 32);
+    if (w0 + n32 >= r1) return;                                            // rows past the tile's last one repeat it
+    if (parts == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        T *dst = (T *)a.out + (rq.q0 + tok) * a.o_row + hq * a.o_head;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = b * 32 + 8 * i + 4 * h;
+                if (e < a.dim) *(V4 *)(dst + e) = V4{(T)(o[b][4 * i] * inv), (T)(o[b][4 * i + 1] * inv), (T)(o[b][4 * i + 2] * inv), (T)(o[b][4 * i + 3] * inv)};
+            }
     } else {
-        if (a.dim <= 64) hipLaunchKernelGGL((paged_attention_kernel<bf16, 8>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((paged_attention_kernel<bf16, 16>), grid, dim3(256), 0, st, a);
+        const long at = ((long)part * a.n_rows + rq.q0 + tok) * (a.hkv * a.group) + hq;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) *(f32x4 *)(ps.o + at * DP + b * 32 + 8 * i + 4 * h) = f32x4{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]};
+        if (h == 0) ps.ml[at] = make_float2(m, l);
+    }
+}
+
+// out = sum over a row's parts, in their order. One wave a (row, query head); the number of parts follows from the lengths as in the
+// kernel that made them (tiles of ROWS packed rows, KEYS keys).
+template <class T, int DP, int ROWS, int KEYS, int LEAST>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, AttnParts ps) {
+    const int lane = threadIdx.x & 63, hqs = a.hkv * a.group;
+    const long id = blockIdx.x * 4L + (threadIdx.x >> 6);
+    const int row = (int)(id / hqs), hq = (int)(id % hqs);
+    if (row >= a.n_rows) return;
+    int lo = 0, hi = a.n_seq;
+    while (lo < hi) { const int x = (lo + hi) >> 1; if (a.cu[x + 1] <= row) lo = x + 1; else hi = x; }
+    if (lo >= a.n_seq || row < a.cu[lo]) return;
+    const AttnReq rq = attn_req(a, lo);
+    const int pr = (row - rq.q0) * a.group + hq % a.group, r0 = pr / ROWS * ROWS, r1 = min(rq.n * a.group, r0 + ROWS);
+    int k0, k1;
+    attn_keys(a, rq, r0, r1, k0, k1);
+    const int n_kt = max((k1 + KEYS - 1) / KEYS - k0 / KEYS, 0), parts = attn_parts(n_kt, ps.splits, LEAST);
+    if (parts == 1) return;                                                // written by the kernel itself
+    const long stride = (long)a.n_rows * hqs, at = (long)row * hqs + hq;
+    float m = -INFINITY, l = 0.0f, acc0 = 0.0f, acc1 = 0.0f;
+    for (int p = 0; p < parts; p++) m = fmaxf(m, ps.ml[p * stride + at].x);
+    for (int p = 0; p < parts; p++) {
+        const float2 ml = ps.ml[p * stride + at];
+        const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
+        l += ml.y * f;
+        const float *src = ps.o + (p * stride + at) * DP + lane * (DP / 64);
+        acc0 += src[0] * f;
+        if (DP == 128) acc1 += src[1] * f;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T *dst = (T *)a.out + row * a.o_row + hq * a.o_head + lane * (DP / 64);
+    if (lane * (DP / 64) < a.dim) { dst[0] = (T)(acc0 * inv); if (DP == 128) dst[1] = (T)(acc1 * inv); }
+}
+
+// How a call is cut up. The step kernel takes calls whose requests bring at most 16 packed rows each, as far as the caller says;
+// it is right for any, 16 rows at a time.
+struct AttnShape { bool step; int tiles, splits; };
+static AttnShape attn_shape(const PagedAttn &a) {
+    AttnShape s;
+    const long new_rows = (long)(a.max_new > 0 ? a.max_new : a.n_rows) * a.group, keys = a.max_kv > 0 ? a.max_kv : 0x7fffffff;
+    s.step = new_rows <= kStepRows;
+    s.tiles = s.step ? a.n_seq : (int)((long)a.n_rows * a.group / kChunkRows + a.n_seq);
+    const long work = (long)s.tiles * a.hkv, full = s.step ? 2048 : 1024, least = s.step ? kStepLeast * kStepKeys : kChunkLeast * kChunkKeys;
+    long n = (full + work - 1) / work;
+    if (n > keys / least) n = keys / least;
+    s.splits = n < 1 ? 1 : n > 256 ? 256 : (int)n;
+    return s;
+}
+
+size_t paged_attention_workspace(const PagedAttn &a) {
+    if (a.n_rows == 0 || a.n_seq == 0) return 0;
+    const AttnShape s = attn_shape(a);
+    const size_t each = (size_t)s.splits * a.n_rows * a.hkv * a.group;
+    return s.splits == 1 ? 0 : each * ((a.dim <= 64 ? 64 : 128) * sizeof(float) + sizeof(float2));
+}
+
+template <class T, int DP> static bool attn_launch(const PagedAttn &a, void *workspace, hipStream_t st) {
+    const AttnShape s = attn_shape(a);
+    const long pairs = (long)a.n_rows * a.hkv * a.group;
+    const AttnParts ps{(float *)workspace, (float2 *)((float *)workspace + (s.splits == 1 ? 0 : s.splits * pairs * DP)), s.splits};
+    const unsigned join = (unsigned)((pairs + 3) / 4);
+    if (s.step) {
+        const dim3 grid((unsigned)(a.n_seq * a.hkv), s.splits);
+        if (a.lp >= 4) hipLaunchKernelGGL((paged_step_kernel<T, DP, true>), grid, dim3(256), 0, st, a, ps);
+        else hipLaunchKernelGGL((paged_step_kernel<T, DP, false>), grid, dim3(256), 0, st, a, ps);
+        if (s.splits > 1) hipLaunchKernelGGL((paged_join_kernel<T, DP, kStepRows, kStepKeys, kStepLeast>), dim3(join), dim3(256), 0, st, a, ps);
+    } else {
+        hipLaunchKernelGGL((paged_chunk_kernel<T, DP>), dim3((unsigned)((long)s.tiles * a.hkv * s.splits)), dim3(256), 0, st, a, ps, s.tiles);
+        if (s.splits > 1) hipLaunchKernelGGL((paged_join_kernel<T, DP, kChunkRows, kChunkKeys, kChunkLeast>), dim3(join), dim3(256), 0, st, a, ps);
     }
     return hipGetLastError() == hipSuccess;
+}
+
+bool paged_attention(const PagedAttn &a, void *workspace, hipStream_t st) {
+    if (a.dtype == WMI_F16) return a.dim <= 64 ? attn_launch<f16, 64>(a, workspace, st) : attn_launch<f16, 128>(a, workspace, st);
+    return a.dim <= 64 ? attn_launch<bf16, 64>(a, workspace, st) : attn_launch<bf16, 128>(a, workspace, st);
 }
 
 namespace {
@@ -236,7 +742,8 @@ int fill_attn(const wmi_paged_cache *c, const wmi_paged_attn *p, PagedAttn &a) {
     if (rc) return rc;
     if (!p || p->n_rows < 0 || p->n_seq < 0 || p->n_q_heads < 1 || p->n_q_heads % c->n_kv_heads || p->table_cols < 0 || p->window < 0 || p->max_new < 0 || p->max_kv < 0) return -1;
     if (!(p->scale == p->scale) || p->scale - p->scale != 0.0f) return -1;          // NaN or infinite
-    if (c->head_dim % 8 || c->head_dim > 128 || p->n_q_heads / c->n_kv_heads > 128 || c->n_kv_heads > 65535) return -3;
+    if (c->head_dim % 8 || c->head_dim > 128 || p->n_q_heads / c->n_kv_heads > 128) return -3;
+    if ((long long)p->n_rows * p->n_q_heads > 0x3fffffffLL || (long long)p->n_seq * c->n_kv_heads > 0x3fffffLL) return -3;      // workgroup and packed row numbers are 32-bit
     a.k = c->k; a.v = c->v; a.dtype = c->dtype; a.n_pages = c->n_pages; a.lp = log2_of(c->page_tokens); a.hkv = c->n_kv_heads; a.dim = c->head_dim;
     a.page_stride = c->page_stride; a.token_stride = c->token_stride; a.head_stride = c->head_stride;
     a.group = p->n_q_heads / c->n_kv_heads; a.n_rows = p->n_rows; a.n_seq = p->n_seq; a.cols = p->table_cols; a.table_stride = p->table_stride;
