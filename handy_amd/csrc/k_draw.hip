@@ -6,24 +6,29 @@ namespace wmi {
 
 // Weights w_i = exp((x_i - max x) / T) lie in [0, 1]. They are computed in 64 bits and rounded to whole numbers of 2^-45: sums of up to
 // 2^18 of them fit 64 bits and are exact, so they do not depend on the order in which they are made (nor on which workgroup shape
-// made them), and every comparison of running masses (top-p's border, the draw) is exact. A weight's rounding costs 2^-46 of the
-// largest one: a draw nearer than that to a border may fall on its other side.
+// made them), and every comparison of running masses (top-p's border, the draw) is exact. What the rounding of a weight costs is
+// 2^-46 of the largest one: a draw nearer than that to a border may fall on its other side.
 // The filters keep a prefix of the order (x descending, index ascending). It is described by a value, the cut: entries above it are
 // kept, and of the entries equal to it the first few by index.
-//   1. the row's largest and lowest finite value
-//   2. all weights: the whole mass (for the log-probability) and, with top-k or top-p, counts and masses in kDrawBins bins of equal
-//      width from the largest value down
-//   3. the cut lies in the first bin whose running count (mass) reaches what is asked for: its members, mostly a few dozen, are
-//      collected and ranked; crowded bins are resolved by radix selection instead
-//   4. the kept mass of every wave's run of the vocabulary, then of the run that holds the draw, a few entries a thread
-// One workgroup a row. Every pass reads the row again: it comes from HBM once and from the caches afterwards.
+// One workgroup a row; the row comes from HBM once and out of the caches in later passes:
+//   1. the largest value
+//   2. the whole mass (for the log-probability; without a filter also what the draw needs, by wave)
+//   3. the cut. A short top-k or min_p alone: the k-th largest of the threads' own maxima (at least k entries reach it) or the border
+//      weight bounds it from below; the entries that reach the bound are listed in the LDS, and the rest of the work runs over the list. Other
+//      filters (and lists that overflow): pass 2 also adds counts and masses up in kDrawBins bins of equal width from the largest
+//      value down, masses by wave; the cut lies in the first bin whose running sum reaches what is asked for. Either way that bin's
+//      members are ranked, or resolved by radix selection if there are many.
+//   4. the draw, in the vocabulary's order: the wave's run that holds it, the thread's few entries, the entry.
+// Bound by 64-bit arithmetic (pass 2: 21 such instructions a weight, about 7 us for 51866 entries on one compute unit) and by the waits
+// of the short steps, which a second row on the same compute unit covers.
 constexpr double kMassOne = 35184372088832.0;               // 2^45
-constexpr int kDrawBins = 2048, kDrawList = 128, kDrawSmall = 16384;
+constexpr int kDrawBins = 768, kDrawRank = 1024, kDrawClose = 128, kDrawCap = 1024;
 
 typedef unsigned long long u64;
 
 __device__ __forceinline__ u64 wave_sum64(u64 v) { for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o); return v; }
 __device__ __forceinline__ u64 wave_scan64(u64 v, int lane) { for (int o = 1; o < 64; o <<= 1) { const u64 y = __shfl_up(v, o); if (lane >= o) v += y; } return v; }
+__device__ __forceinline__ unsigned wave_scan32(unsigned v, int lane) { for (int o = 1; o < 64; o <<= 1) { const unsigned y = __shfl_up(v, o); if (lane >= o) v += y; } return v; }
 
 // unsigned order of floats (no NaN, no -0): key(a) < key(b) <=> a < b
 __device__ __forceinline__ unsigned draw_key(float x) { const unsigned u = __float_as_uint(x); return u & 0x80000000u ? ~u : u | 0x80000000u; }
@@ -32,9 +37,9 @@ __device__ __forceinline__ float draw_val(unsigned k) { return __uint_as_float(k
 // weights relative to a row's largest value `top`
 struct DrawScale {
     double top, s;                                           // s = log2(e) / T
-    // 2^((x - top) s), rounded to a multiple of 2^-45: 2^f on [-1/2, 1/2] by a polynomial (Chebyshev interpolation, 2^-51 relative),
-    // the exponent by ldexp; adding 128 leaves 45 bits behind the point
-    __device__ __forceinline__ double weight(float x) const {
+    // 2^((x - top) s): 2^f on [-1/2, 1/2] by a polynomial (Chebyshev interpolation, 2^-51 relative), its exponent moved by the whole
+    // part (never below 2^-1001)
+    __device__ __forceinline__ double exact(float x) const {
         const double y = fmax(((double)x - top) * s, -1000.0), t = y + 6755399441055744.0, f = y - (t - 6755399441055744.0);
         double p = 0x1.e6064532b85cep-28;
         p = __builtin_fma(p, f, 0x1.b675bd731322bp-24);
@@ -47,9 +52,11 @@ struct DrawScale {
         p = __builtin_fma(p, f, 0x1.ebfbdff82c598p-3);
         p = __builtin_fma(p, f, 0x1.62e42fefa3a19p-1);
         p = __builtin_fma(p, f, 1.0);
-        return (__builtin_amdgcn_ldexp(p, (int)__double2loint(t)) + 128.0) - 128.0;
+        return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
     }
-    __device__ __forceinline__ u64 mass(float x) const { return (u64)(weight(x) * kMassOne); }
+    // rounded to a multiple of 2^-45: 128 plus the weight keeps 45 bits behind the point, and is that whole number but for its exponent
+    __device__ __forceinline__ double rounded(float x) const { return exact(x) + 128.0; }
+    __device__ __forceinline__ u64 mass(float x) const { return (u64)__double_as_longlong(rounded(x)) - 0x4060000000000000ull; }
 };
 
 template <class T> struct DrawIn;                            // four consecutive logits at any alignment
@@ -59,87 +66,77 @@ template <> struct DrawIn<__bf16> { typedef __bf16 V __attribute__((ext_vector_t
 
 template <int TH> struct DrawShared {
     static constexpr int W = TH / 64;
-    u64 mass[kDrawBins];                                     // per bin, then running from the largest value down
+    union {
+        u64 hist[W][kDrawBins];                              // masses by wave and bin
+        struct {
+            float list[W][kDrawCap];                         // entries that can be kept, by wave and in order ...
+            unsigned short list_at[W][kDrawCap];             // ... and where in the wave's run (at most 16384 entries) they stand
+        };
+    };
+    u64 mass[kDrawBins];                                     // running from the largest value down
     unsigned count[kDrawBins];
-    u64 list_mass[kDrawList];
-    float list[kDrawList];
-    u64 radix[256];
-    u64 seg_mass[W], wm[W];
-    unsigned seg_ties[W], wc[W];
-    float hi[W], lo[W];
-    u64 above;
-    float cut;
-    unsigned n_list, kmin, kmax, digit, tok;
-    int bin;
+    u64 rank_mass[kDrawRank], radix[256], seg_mass[W], wm[W], above;
+    float rank[kDrawRank], hi[W], lo[W], cut;
+    unsigned seg_ties[W], wc[W], n_listed[W], n_member[W];
+    unsigned n_rank, kmin, kmax, digit, tok, walk_rank;
+    unsigned n_close;
+    int bin, walk_at;
+    unsigned short close[kDrawClose];
+    unsigned char rank_wave[kDrawRank];
 };
 
 template <class T, int TH>
-__global__ __launch_bounds__(TH) void draw_kernel(DrawArgs a) {
+__global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
     typedef typename DrawIn<T>::V V4;
     constexpr int W = TH / 64, U = 4;
     __shared__ DrawShared<TH> sh;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), V = a.n_vocab;
     const T *src = (const T *)a.logits + row * a.row_stride;
+    const float t_in = a.temperature ? a.temperature[row] : 1.0f, p_in = a.top_p ? a.top_p[row] : 1.0f, m_in = a.min_p ? a.min_p[row] : 0.0f, u_in = a.uniform[row];
+    const int k_in = a.top_k ? a.top_k[row] : 0;
     const int run = ((V + W - 1) / W + 255) & ~255;          // entries of a wave
     const int base = min(V, wave * run), lim = min(V, base + run);
     auto clean = [](float v) { return fmaxf(v + 0.0f, -INFINITY); };               // -0 -> +0, NaN -> -infinity
-    // one pass over the row: body(x, i) for every entry of this wave; past the end it sees -infinity (the wave stays whole)
-    auto pass = [&](auto body) __attribute__((always_inline)) {
+    // one pass over the row, four entries a lane at a time: body(x[4], i) for entries i .. i + 3 (-infinity past the wave's end; the
+    // wave stays whole)
+    auto stream4 = [&](auto body) __attribute__((always_inline)) {
         for (int b = base; b < lim; b += 256 * U) {
-            float x[4 * U];
+            float y[4 * U];
 #pragma unroll
             for (int j = 0; j < U; j++) {
                 const int i = b + 256 * j + lane * 4;
                 if (i + 4 <= lim) {
                     const V4 v = *(const V4 *)(src + i);
 #pragma unroll
-                    for (int c = 0; c < 4; c++) x[4 * j + c] = (float)v[c];
+                    for (int c = 0; c < 4; c++) y[4 * j + c] = (float)v[c];
                 } else {
 #pragma unroll
-                    for (int c = 0; c < 4; c++) x[4 * j + c] = i + c < lim ? (float)src[i + c] : -INFINITY;
+                    for (int c = 0; c < 4; c++) y[4 * j + c] = i + c < lim ? (float)src[i + c] : -INFINITY;
                 }
             }
 #pragma unroll
             for (int j = 0; j < U; j++) {
                 if (b + 256 * j >= lim) break;               // uniform
 #pragma unroll
-                for (int c = 0; c < 4; c++) body(clean(x[4 * j + c]), b + 256 * j + lane * 4 + c);
+                for (int c = 0; c < 4; c++) y[4 * j + c] = clean(y[4 * j + c]);
+                body(y + 4 * j, b + 256 * j + lane * 4);
             }
         }
     };
-
-    // 1. largest and lowest finite value
-    float top = -INFINITY, low = INFINITY;
-    pass([&](float x, int) { top = fmaxf(top, x); low = fminf(low, x == -INFINITY ? INFINITY : x); });
-    for (int o = 32; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor(top, o)); low = fminf(low, __shfl_xor(low, o)); }
-    if (lane == 0) { sh.hi[wave] = top; sh.lo[wave] = low; }
-    __syncthreads();
+    bool listed = false;
+    // one pass over what can be kept: body(x, i) for every entry i of this wave's part of the list, or of the row
+    auto pass = [&](auto body) __attribute__((always_inline)) {
+        if (listed) {
+            const int n = (int)sh.n_listed[wave];
+            for (int j0 = 0; j0 < n; j0 += 64) {
+                const bool on = j0 + lane < n;
+                body(on ? sh.list[wave][j0 + lane] : -INFINITY, on ? base + (int)sh.list_at[wave][j0 + lane] : 0);
+            }
+        } else stream4([&](const float *v, int i) {
 #pragma unroll
-    for (int w = 0; w < W; w++) { top = fmaxf(top, sh.hi[w]); low = fminf(low, sh.lo[w]); }
-    if (top == -INFINITY) {                                  // nothing can be drawn
-        if (tid == 0) { a.token[row] = -1; if (a.logprob) a.logprob[row] = -INFINITY; }
-        return;
-    }
-    const float t_in = a.temperature ? a.temperature[row] : 1.0f;
-    const bool drawn = t_in > 0.0f;
-    const double T64 = drawn ? (double)t_in : 1.0;
-    const DrawScale sc{(double)top, 1.4426950408889634 / T64};
-    const int top_k = drawn && a.top_k ? a.top_k[row] : 0;
-    const float top_p = drawn && a.top_p ? a.top_p[row] : 1.0f, min_p = drawn && a.min_p ? a.min_p[row] : 0.0f;
-    const bool use_k = top_k > 0 && top_k < V, use_p = top_p < 1.0f, use_m = min_p > 0.0f;
-
-    const u64 top_m = (u64)kMassOne;
-    auto mass_of = [&](float x) { return x == top ? top_m : sc.mass(x); };           // (an infinite largest value has no difference to itself)
-    float cut = -INFINITY;
-    unsigned ties = 0;
-    u64 z;
-
-    // 2. masses, and the histogram. Bins of equal width from the largest value down, in halves so that no difference overflows; with
-    // top-p alone they need not reach below the values whose mass is 0.
-    float floor_v = low;
-    if (use_p && !use_k) floor_v = fmaxf(low, (float)((double)top - 32.0 * T64));
-    const float half_top = 0.5f * top, width = half_top - 0.5f * floor_v, per_bin = width > 0.0f ? (float)kDrawBins / width : 0.0f;
-    auto bin_of = [&](float v) { return (int)fminf((half_top - 0.5f * v) * per_bin, (float)(kDrawBins - 1)); };
+            for (int c = 0; c < 4; c++) body(v[c], i + c);
+        });
+    };
     auto block_sum = [&](u64 s) -> u64 {
         s = wave_sum64(s);
         __syncthreads();
@@ -150,33 +147,122 @@ __global__ __launch_bounds__(TH) void draw_kernel(DrawArgs a) {
         for (int w = 0; w < W; w++) t += sh.wm[w];
         return t;
     };
-    // the value at which the running count (by_mass: mass) from the largest value down reaches want > 0, and the sum over larger values
+
+    // 1. largest and lowest finite value
+    float top = -INFINITY, low = INFINITY;
+    stream4([&](const float *v, int) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) { top = fmaxf(top, v[c]); low = fminf(low, v[c] == -INFINITY ? INFINITY : v[c]); }
+    });
+    const float own_top = top;
+    for (int o = 32; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor(top, o)); low = fminf(low, __shfl_xor(low, o)); }
+    if (lane == 0) { sh.hi[wave] = top; sh.lo[wave] = low; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; w++) { top = fmaxf(top, sh.hi[w]); low = fminf(low, sh.lo[w]); }
+    if (top == -INFINITY) {                                  // nothing can be drawn
+        if (tid == 0) { a.token[row] = -1; if (a.logprob) a.logprob[row] = -INFINITY; }
+        return;
+    }
+    const bool drawn = t_in > 0.0f;
+    const double T64 = drawn ? (double)t_in : 1.0;
+    const DrawScale sc{(double)top, 1.4426950408889634 / T64};
+    const int top_k = drawn ? k_in : 0;
+    const float top_p = drawn ? p_in : 1.0f, min_p = drawn ? m_in : 0.0f;
+    const bool use_k = top_k > 0 && top_k < V, use_p = top_p < 1.0f, use_m = min_p > 0.0f;
+    const u64 top_m = (u64)kMassOne;
+    auto mass_of = [&](float v) { return v == top ? top_m : sc.mass(v); };           // (an infinite largest value has no difference to itself)
+    float cut = -INFINITY;
+    unsigned ties = 0;
+    u64 z = 0;
+
+    // bins of equal width from the largest value down to floor_v, in halves so that no difference overflows
+    const float half_top = 0.5f * top;
+    float per_bin = 0.0f;
+    auto set_bins = [&](float floor_v) { const float width = half_top - 0.5f * floor_v; per_bin = width > 0.0f ? (float)kDrawBins / width : 0.0f; };
+    auto bin_of = [&](float v) { return (int)fminf((half_top - 0.5f * v) * per_bin, (float)(kDrawBins - 1)); };
+    // running sums over the bins, in place
+    auto run_bins = [&]() __attribute__((always_inline)) {
+        constexpr int B = (kDrawBins + TH - 1) / TH;
+        const int b0 = min(kDrawBins, tid * B), b1 = min(kDrawBins, b0 + B);
+        u64 m = 0;
+        unsigned c = 0;
+        for (int i = b0; i < b1; i++) { m += sh.mass[i]; c += sh.count[i]; }
+        u64 xm = wave_scan64(m, lane);
+        unsigned xc = wave_scan32(c, lane);
+        __syncthreads();
+        if (lane == 63) { sh.wm[wave] = xm; sh.wc[wave] = xc; }
+        __syncthreads();
+        xm -= m; xc -= c;
+        for (int w = 0; w < wave; w++) { xm += sh.wm[w]; xc += sh.wc[w]; }
+        for (int i = b0; i < b1; i++) { xm += sh.mass[i]; sh.mass[i] = xm; xc += sh.count[i]; sh.count[i] = xc; }
+        __syncthreads();
+    };
+    auto clear_bins = [&]() { for (int i = tid; i < kDrawBins; i += TH) { sh.count[i] = 0; sh.mass[i] = 0; } };
+    // the digit (of 256, from the highest down) in which `sum` and the digits' measures reach want, by wave 0
+    auto pick_digit = [&](u64 want, u64 sum) {
+        if (wave == 0) {                                     // lane l: digits 255 - 4 l and the three below
+            u64 d[4], t = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) { d[i] = sh.radix[255 - 4 * lane - i]; t += d[i]; }
+            u64 r = sum + wave_scan64(t, lane) - t;
+#pragma unroll
+            for (int i = 0; i < 4; i++) { if (r < want && r + d[i] >= want) { sh.digit = 255 - 4 * lane - i; sh.above = r; } r += d[i]; }
+        }
+        __syncthreads();
+    };
+    // the same as select among n collected members: 256 bins of equal width between the lowest and the highest, then the members of
+    // one of them, each against each. False: too many fall into that bin
+    auto narrow = [&](u64 want, bool by_mass, int n, u64 above) -> bool {
+        const float lo = draw_val(sh.kmin), per = 255.99f / (0.5f * draw_val(sh.kmax) - 0.5f * lo);
+        auto digit_of = [&](float v) { return (unsigned)fminf((0.5f * v - 0.5f * lo) * per, 255.0f); };
+        for (int i = tid; i < 256; i += TH) sh.radix[i] = 0;
+        if (tid == 0) sh.n_close = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += TH) { const u64 m = by_mass ? sh.rank_mass[i] : 1; if (m) atomicAdd(&sh.radix[digit_of(sh.rank[i])], m); }
+        __syncthreads();
+        pick_digit(want, above);
+        const unsigned digit = sh.digit;
+        const u64 base_sum = sh.above;
+        for (int i = tid; i < n; i += TH)
+            if (digit_of(sh.rank[i]) == digit) { const unsigned at = atomicAdd(&sh.n_close, 1u); if (at < (unsigned)kDrawClose) sh.close[at] = (unsigned short)i; }
+        __syncthreads();
+        const int k = (int)sh.n_close;
+        if (k > kDrawClose) return false;
+        if (tid < k) {
+            const float v = sh.rank[sh.close[tid]];
+            u64 gt = base_sum, eq = 0;
+            for (int j = 0; j < k; j++) { const int at = sh.close[j]; const float o = sh.rank[at]; const u64 m = by_mass ? sh.rank_mass[at] : 1; if (o > v) gt += m; else if (o == v) eq += m; }
+            if (gt < want && gt + eq >= want) { sh.cut = v; sh.above = gt; }              // the members of one value agree
+        }
+        __syncthreads();
+        return true;
+    };
+    // the value at which the running count (by_mass: mass) from the largest value down reaches want > 0, and the sum over larger
+    // values. Leaves what it collected of that bin: sh.bin, sh.n_rank, sh.kmin, sh.kmax, sh.n_member, sh.rank*
     auto select = [&](u64 want, bool by_mass, float &v_out, u64 &above_out) __attribute__((always_inline)) {
         auto running = [&](int b) -> u64 { return b < 0 ? 0 : by_mass ? sh.mass[b] : (u64)sh.count[b]; };
-        if (tid == 0) { sh.n_list = 0; sh.kmin = 0xffffffffu; sh.kmax = 0; }
+        if (tid == 0) { sh.n_rank = 0; sh.kmin = 0xffffffffu; sh.kmax = 0; }
         for (int i = tid; i < kDrawBins; i += TH) if (running(i) >= want && running(i - 1) < want) sh.bin = i;
         __syncthreads();
         const int bin = sh.bin;
         const u64 above = running(bin - 1);
+        unsigned members = 0, kmin = 0xffffffffu, kmax = 0;
         pass([&](float x, int) {
             if (x != -INFINITY && bin_of(x) == bin) {
-                const unsigned at = atomicAdd(&sh.n_list, 1u), key = draw_key(x);
-                atomicMin(&sh.kmin, key); atomicMax(&sh.kmax, key);
-                if (at < (unsigned)kDrawList) { sh.list[at] = x; sh.list_mass[at] = by_mass ? mass_of(x) : 1; }
+                const unsigned at = atomicAdd(&sh.n_rank, 1u), key = draw_key(x);
+                kmin = min(kmin, key); kmax = max(kmax, key);
+                members++;
+                if (at < (unsigned)kDrawRank) { sh.rank[at] = x; sh.rank_mass[at] = mass_of(x); sh.rank_wave[at] = (unsigned char)wave; }
             }
         });
+        for (int o = 32; o > 0; o >>= 1) { members += __shfl_xor(members, o); kmin = min(kmin, (unsigned)__shfl_xor(kmin, o)); kmax = max(kmax, (unsigned)__shfl_xor(kmax, o)); }
+        if (lane == 0 && members) { atomicMin(&sh.kmin, kmin); atomicMax(&sh.kmax, kmax); }
+        if (lane == 0) sh.n_member[wave] = members;
         __syncthreads();
-        const int n = (int)sh.n_list;
+        const int n = (int)sh.n_rank;
         if (sh.kmin == sh.kmax) { v_out = draw_val(sh.kmin); above_out = above; }
-        else if (n <= kDrawList) {                           // every member looks at every other
-            if (tid < n) {
-                const float v = sh.list[tid];
-                u64 gt = above, eq = 0;
-                for (int j = 0; j < n; j++) { const float o = sh.list[j]; const u64 m = sh.list_mass[j]; if (o > v) gt += m; else if (o == v) eq += m; }
-                if (gt < want && gt + eq >= want) { sh.cut = v; sh.above = gt; }          // the members of one value agree
-            }
-            __syncthreads();
-            v_out = sh.cut; above_out = sh.above;
+        else if (n <= kDrawRank && narrow(want, by_mass, n, above)) { v_out = sh.cut; above_out = sh.above;
         } else {                                             // radix selection among the members, 8 bits of the key at a time
             unsigned prefix = 0;
             u64 sum = above;
@@ -191,15 +277,7 @@ __global__ __launch_bounds__(TH) void draw_kernel(DrawArgs a) {
                     }
                 });
                 __syncthreads();
-                if (wave == 0) {                             // lane l: digits 255 - 4 l and the three below
-                    u64 d[4], t = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) { d[i] = sh.radix[255 - 4 * lane - i]; t += d[i]; }
-                    u64 r = sum + wave_scan64(t, lane) - t;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) { if (r < want && r + d[i] >= want) { sh.digit = 255 - 4 * lane - i; sh.above = r; } r += d[i]; }
-                }
-                __syncthreads();
+                pick_digit(want, sum);
                 prefix |= sh.digit << shift;
                 sum = sh.above;
             }
@@ -209,62 +287,138 @@ __global__ __launch_bounds__(TH) void draw_kernel(DrawArgs a) {
     };
 
     if (top == INFINITY) {                                   // infinite entries share everything: the cut is among them
-        u64 n = 0;
-        pass([&](float x, int) { n += x == INFINITY; });
-        n = block_sum(n);
-        z = n * top_m;
+        unsigned n = 0;
+        stream4([&](const float *v, int) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) n += v[c] == INFINITY;
+        });
+        const unsigned all = (unsigned)block_sum(n);         // (a wave's sum of lanes, then of waves)
+        for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+        if (lane == 0) { sh.seg_mass[wave] = 0; sh.seg_ties[wave] = n; }
+        z = all * top_m;
         cut = top;
-        ties = drawn ? (unsigned)n : 1;
+        ties = drawn ? all : 1;
         if (use_k && ties > (unsigned)top_k) ties = (unsigned)top_k;
         if (use_p) { const double l = ceil((double)top_p * (double)ties); ties = l > 1.0 ? (unsigned)l : 1; }
         if (use_m && min_p > 1.0f) ties = 1;
     } else {
-        const bool hist = use_k || use_p;
-        if (hist) {
-            for (int i = tid; i < kDrawBins; i += TH) { sh.count[i] = 0; sh.mass[i] = 0; }
+        const bool filtered = !drawn || use_k || use_p || use_m;
+        bool binned = drawn && (use_k ? top_k > TH / 2 : use_p);
+#pragma clang loop unroll(disable)
+        for (;;) {
+            if (binned) {
+                // without top-k the bins need not reach below the values whose mass is 0
+                set_bins(use_k ? low : fmaxf(low, (float)((double)top - 32.0 * T64)));
+                clear_bins();
+                for (int i = tid; i < W * kDrawBins; i += TH) (&sh.hist[0][0])[i] = 0;
+                __syncthreads();
+            }
+            // 2. the whole mass
+            double acc = 0.0;                                // at most 256 multiples of 2^-45 up to 1: exact
+            if (!binned) stream4([&](const float *v, int) {
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc += sc.rounded(v[c]) - 128.0;
+            });
+            else stream4([&](const float *v, int) {
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const double r = sc.rounded(v[c]);
+                    const u64 m = (u64)__double_as_longlong(r) - 0x4060000000000000ull;
+                    const int b = bin_of(v[c]);
+                    acc += r - 128.0;
+                    if (use_k && v[c] != -INFINITY) atomicAdd(&sh.count[b], 1u);
+                    if (m) atomicAdd(&sh.hist[wave][b], m);
+                }
+            });
+            const u64 own = wave_sum64((u64)(acc * kMassOne));
+            if (lane == 0) { sh.seg_mass[wave] = own; sh.seg_ties[wave] = 0; }
+            __syncthreads();
+            z = 0;
+#pragma unroll
+            for (int w = 0; w < W; w++) z += sh.seg_mass[w];
+            if (!filtered || binned) break;
+
+            // 3. the list: entries from the bin on that holds the k-th largest of the threads' maxima -- from the lowest maximum in it
+            float least = top;
+            if (drawn && !use_k) least = fminf(top, (float)((double)top + T64 * (log(fmin((double)min_p, 1.0)) - 1e-6)));       // (a slack far beyond every rounding here)
+            else if (drawn) {
+                const unsigned kk = (unsigned)top_k;
+                clear_bins();
+                set_bins(low);
+                const int mine = own_top == -INFINITY ? kDrawBins : bin_of(own_top);
+                if (tid == 0) { sh.bin = kDrawBins; sh.kmin = 0xffffffffu; }
+                __syncthreads();
+                if (mine < kDrawBins) atomicAdd(&sh.count[mine], 1u);
+                __syncthreads();
+                run_bins();
+                for (int i = tid; i < kDrawBins; i += TH) if (sh.count[i] >= kk && (i == 0 || sh.count[i - 1] < kk)) sh.bin = i;
+                __syncthreads();
+                const int upto = sh.bin;                     // (kDrawBins: fewer than k threads hold anything -- everything is listed)
+                if (mine <= upto && mine < kDrawBins) atomicMin(&sh.kmin, draw_key(own_top));
+                __syncthreads();
+                least = upto < kDrawBins ? draw_val(sh.kmin) : low;
+            }
+            unsigned n = 0;
+            stream4([&](const float *v, int i) {
+                u64 has[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) has[j] = __ballot(v[j] >= least);
+                if ((has[0] | has[1] | has[2] | has[3]) != 0) {          // a lane's four entries come one after the other
+                    unsigned at = n;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) { at += __builtin_amdgcn_mbcnt_hi((unsigned)(has[j] >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)has[j], 0)); n += __popcll(has[j]); }
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (v[j] >= least) {
+                            if (at < (unsigned)kDrawCap) { sh.list[wave][at] = v[j]; sh.list_at[wave][at] = (unsigned short)(i + j - base); }
+                            at++;
+                        }
+                }
+            });
+            if (lane == 0) sh.n_listed[wave] = n;
+            __syncthreads();
+            listed = true;
+#pragma unroll
+            for (int w = 0; w < W; w++) listed &= sh.n_listed[w] <= (unsigned)kDrawCap;
+            if (listed) {
+                if (use_k) {
+                    set_bins(least);
+                    clear_bins();
+                    __syncthreads();
+                    pass([&](float v, int) {
+                        if (v != -INFINITY) {
+                            const int b = bin_of(v);
+                            atomicAdd(&sh.count[b], 1u);
+                            if (use_p) { const u64 m = sc.mass(v); if (m) atomicAdd(&sh.mass[b], m); }
+                        }
+                    });
+                }
+                break;
+            }
+            binned = true;
             __syncthreads();
         }
-        double acc = 0.0;                                    // at most 256 multiples of 2^-45 up to 1: exact
-        pass([&](float x, int) {
-            const double w = sc.weight(x);
-            acc += w;
-            if (hist && x != -INFINITY) {
-                const int b = bin_of(x);
-                if (use_k) atomicAdd(&sh.count[b], 1u);
-                if (use_p && w > 0.0) atomicAdd(&sh.mass[b], (u64)(w * kMassOne));
-            }
-        });
-        const u64 own = wave_sum64((u64)(acc * kMassOne));
-        if (lane == 0) { sh.seg_mass[wave] = own; sh.seg_ties[wave] = 0; }
-        __syncthreads();
-        z = 0;
-#pragma unroll
-        for (int w = 0; w < W; w++) z += sh.seg_mass[w];
 
         // 3. the cut
-        if (hist) {                                          // running sums over the bins, in place
-            constexpr int B = kDrawBins / TH;
-            u64 m = 0;
-            unsigned c = 0;
-#pragma unroll
-            for (int i = 0; i < B; i++) { m += sh.mass[tid * B + i]; c += sh.count[tid * B + i]; }
-            u64 xm = wave_scan64(m, lane);
-            unsigned xc = c;
-            for (int o = 1; o < 64; o <<= 1) { const unsigned y = __shfl_up(xc, o); if (lane >= o) xc += y; }
-            if (lane == 63) { sh.wm[wave] = xm; sh.wc[wave] = xc; }
-            __syncthreads();
-            xm -= m; xc -= c;
-            for (int w = 0; w < wave; w++) { xm += sh.wm[w]; xc += sh.wc[w]; }
-#pragma unroll
-            for (int i = 0; i < B; i++) { xm += sh.mass[tid * B + i]; sh.mass[tid * B + i] = xm; xc += sh.count[tid * B + i]; sh.count[tid * B + i] = xc; }
-            __syncthreads();
-        }
         if (!drawn) { cut = top; ties = 1; }
+        else if (use_k || use_p) {
+            if (binned) {
+                for (int i = tid; i < kDrawBins; i += TH) {
+                    u64 m = 0;
+#pragma unroll
+                    for (int w = 0; w < W; w++) m += sh.hist[w][i];
+                    sh.mass[i] = m;
+                }
+            }
+            __syncthreads();
+            run_bins();
+        }
+        bool ranked = false;                                 // select has run: its bin's members are known
 #pragma clang loop unroll(disable)
         for (int by_mass = 0; by_mass < 2; by_mass++) {      // top-k by counts, then top-p by masses
             u64 want;
             if (!by_mass) {
-                if (!use_k || (unsigned)top_k >= sh.count[kDrawBins - 1]) continue;
+                if (!use_k || (unsigned)top_k > sh.count[kDrawBins - 1]) continue;
                 want = (u64)top_k;
             } else {
                 // rank j is kept while the mass before it is < top_p * mass of the first k, that is < want; the first always is
@@ -281,6 +435,7 @@ __global__ __launch_bounds__(TH) void draw_kernel(DrawArgs a) {
             float v;
             u64 above;
             select(want, by_mass != 0, v, above);
+            ranked = true;
             if (!by_mass) { cut = v; ties = (unsigned)(want - above); }
             else if (ties == 0 || v >= cut) {
                 const u64 w = mass_of(v), t = (want - above + w - 1) / w;
@@ -294,7 +449,7 @@ __global__ __launch_bounds__(TH) void draw_kernel(DrawArgs a) {
             const double m64 = (double)min_p;
             while (n > 0) {
                 const unsigned step = n / 64 + 1, at = lane * step;
-                const bool light = at < n && !(exp(((double)draw_val(lo + at) - (double)top) / T64) >= m64);       // the answer lies behind
+                const bool light = at < n && !(sc.exact(draw_val(lo + at)) >= m64);       // the answer lies behind
                 const unsigned k = __popcll(__ballot(light));
                 if (k == 0) break;
                 lo += (k - 1) * step + 1;
@@ -304,11 +459,36 @@ __global__ __launch_bounds__(TH) void draw_kernel(DrawArgs a) {
             if (v > top) { cut = top; ties = 1; }            // (the first always is)
             else if (v > cut) { cut = draw_val(lo - 1); ties = 0; }
         }
+        // masses above the cut and entries equal to it, by wave (without a cut: pass 2's)
+        if (cut > -INFINITY) {
+            u64 s = 0;
+            unsigned t = 0;
+            const int bin = binned ? bin_of(cut) : -1;
+            if (binned && ranked && bin == sh.bin && (sh.n_rank <= (unsigned)kDrawRank || sh.kmin == sh.kmax)) {
+                for (int i = lane; i < bin; i += 64) s += sh.hist[wave][i];
+                if (sh.kmin == sh.kmax) t = lane == 0 && draw_val(sh.kmin) == cut ? sh.n_member[wave] : 0;
+                if (sh.kmin != sh.kmax || draw_val(sh.kmin) > cut)
+                    for (int j = lane; j < (int)min(sh.n_rank, (unsigned)kDrawRank); j += 64)
+                        if (sh.rank_wave[j] == wave) { if (sh.rank[j] > cut) s += sh.rank_mass[j]; else t += sh.rank[j] == cut; }
+            } else {
+                if (binned) for (int i = lane; i < bin; i += 64) s += sh.hist[wave][i];
+                pass([&](float x, int) {
+                    const bool here = !binned || bin_of(x) == bin;       // (the bins before hold only entries above the cut)
+                    if (__any(here && x > cut)) s += here && x > cut ? mass_of(x) : 0;
+                    t += x == cut;
+                });
+            }
+            s = wave_sum64(s);
+            for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
+            __syncthreads();
+            if (lane == 0) { sh.seg_mass[wave] = s; sh.seg_ties[wave] = t; }
+        }
     }
 
     // 4. the draw, in the vocabulary's order
     const u64 cut_m = ties ? mass_of(cut) : 0;
-    const double u = fmin(a.uniform[row] > 0.0f ? (double)a.uniform[row] : 0.0, 1.0 - 0x1p-24);
+    const double u = fmin(u_in > 0.0f ? (double)u_in : 0.0, 1.0 - 0x1p-24);
+    __syncthreads();
     if (u == 0.0) {                                          // the first kept entry of any weight, below the masses' resolution too
         if (tid == 0) sh.tok = 0xffffffffu;
         __syncthreads();
@@ -318,60 +498,54 @@ __global__ __launch_bounds__(TH) void draw_kernel(DrawArgs a) {
         });
         if (first != 0xffffffffu) atomicMin(&sh.tok, first);
     } else {
-        if (cut > -INFINITY) {                               // masses above the cut and entries equal to it, by wave
-            u64 s = 0;
-            unsigned t = 0;
-            pass([&](float x, int) {
-                if (__any(x > cut)) s += x > cut ? mass_of(x) : 0;
-                t += x == cut;
-            });
-            s = wave_sum64(s);
-            for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
-            __syncthreads();
-            if (lane == 0) { sh.seg_mass[wave] = s; sh.seg_ties[wave] = t; }
-        }
-        __syncthreads();
         // lane s: the run of wave s
-        const unsigned st = lane < W ? sh.seg_ties[lane] : 0;
-        unsigned tx = st;
-        for (int o = 1; o < 64; o <<= 1) { const unsigned y = __shfl_up(tx, o); if (lane >= o) tx += y; }
-        tx -= st;
-        const unsigned left = ties > tx ? ties - tx : 0;
+        const unsigned st = lane < W ? sh.seg_ties[lane] : 0, tx = wave_scan32(st, lane) - st, left = ties > tx ? ties - tx : 0;
         const u64 sm = lane < W ? sh.seg_mass[lane] + (u64)min(st, left) * cut_m : 0, sums = wave_scan64(sm, lane), total = __shfl(sums, 63);
         const u64 target = (u64)(u * (double)total);         // < total: total >= 2^45
         const int pick = __builtin_ctzll(__ballot(sums > target));
         const u64 before = __shfl(sums - sm, pick);
         const unsigned tie_before = __shfl(tx, pick);
-        const int b = min(V, pick * run), e = min(V, b + run);
-        // that run of the vocabulary, each thread E entries in a row
-        const int E = ((e - b) + TH - 1) / TH, i0 = min(e, b + tid * E), i1 = min(e, i0 + E);
+        // that run of the vocabulary or that part of the list, each thread E entries in a row, loaded 8 at a time
+        const int b = min(V, pick * run), n = listed ? (int)sh.n_listed[pick] : min(V, b + run) - b;
+        const int E = (n + TH - 1) / TH, i0 = min(n, tid * E), i1 = min(n, i0 + E);
+        auto value = [&](int i) { return listed ? sh.list[pick][i] : clean((float)src[b + i]); };
+        auto walk = [&](auto body) __attribute__((always_inline)) {
+            for (int g = i0; g < i1; g += 8) {
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) y[j] = value(min(g + j, i1 - 1));
+#pragma unroll
+                for (int j = 0; j < 8; j++) if (g + j < i1) body(y[j]);
+            }
+        };
         unsigned t = 0;
-        if (ties) for (int i = i0; i < i1; i++) t += clean((float)src[i]) == cut;
-        unsigned ts = t;
-        for (int o = 1; o < 64; o <<= 1) { const unsigned y = __shfl_up(ts, o); if (lane >= o) ts += y; }
+        if (ties) walk([&](float v) { t += v == cut; });
+        unsigned ts = wave_scan32(t, lane);
         if (lane == 63) sh.wc[wave] = ts;
         __syncthreads();
         ts += tie_before - t;
         for (int w = 0; w < wave; w++) ts += sh.wc[w];
-        auto mass_at = [&](int i, unsigned &rank) -> u64 {
-            const float v = clean((float)src[i]);
-            if (v > cut) return mass_of(v);
-            return v == cut && rank++ < ties ? cut_m : 0;
-        };
-        u64 m = 0;
         unsigned rank = ts;
-        for (int i = i0; i < i1; i++) m += mass_at(i, rank);
+        u64 m = 0;
+        walk([&](float v) { m += v > cut ? mass_of(v) : v == cut && rank++ < ties ? cut_m : 0; });
         u64 ms = wave_scan64(m, lane);
         if (lane == 63) sh.wm[wave] = ms;
         __syncthreads();
         ms += before - m;
         for (int w = 0; w < wave; w++) ms += sh.wm[w];
-        if (ms <= target && target < ms + m) {               // one thread
-            rank = ts;
-            u64 c = ms;
-            int i = i0;
-            for (; i < i1 - 1; i++) { c += mass_at(i, rank); if (c > target) break; }
-            sh.tok = (unsigned)i;
+        if (ms <= target && target < ms + m) { sh.walk_at = i0; sh.walk_rank = ts; sh.above = ms; }      // one thread; its entries, one a lane
+        __syncthreads();
+        if (wave == 0) {
+            const int i = sh.walk_at + lane;
+            const bool on = lane < E && i < n;
+            const float v = on ? value(i) : -INFINITY;
+            const u64 eq = __ballot(on && v == cut);
+            const u64 w = !on ? 0 : v > cut ? mass_of(v) : v == cut && sh.walk_rank + __popcll(eq & ((1ull << lane) - 1)) < ties ? cut_m : 0;
+            const u64 hit = __ballot(sh.above + wave_scan64(w, lane) > target);
+            if (lane == 0) {
+                const int at = sh.walk_at + __builtin_ctzll(hit);
+                sh.tok = (unsigned)(b + (listed ? (int)sh.list_at[pick][at] : at));
+            }
         }
     }
     __syncthreads();
@@ -386,8 +560,11 @@ __global__ __launch_bounds__(TH) void draw_kernel(DrawArgs a) {
 }
 
 template <class T> static void draw_launch(const DrawArgs &a, hipStream_t st) {
-    // short rows: four waves a row, so that several rows share a compute unit
-    if (a.n_vocab <= kDrawSmall) hipLaunchKernelGGL((draw_kernel<T, 256>), dim3(a.n_rows), dim3(256), 0, st, a);
+    // Short rows: four waves a row, so that more rows share a compute unit. Else sixteen if every row has a compute unit of its own
+    // (256), or eight, two rows a compute unit, whose waits then fall under the other's arithmetic (1024 rows of 51866 entries: 99 us
+    // against 125). Rows past 131072 always take sixteen: a thread's sum of masses is exact for 256 entries.
+    if (a.n_vocab <= 16384) hipLaunchKernelGGL((draw_kernel<T, 256>), dim3(a.n_rows), dim3(256), 0, st, a);
+    else if (a.n_rows > 256 && a.n_vocab <= 131072) hipLaunchKernelGGL((draw_kernel<T, 512>), dim3(a.n_rows), dim3(512), 0, st, a);
     else hipLaunchKernelGGL((draw_kernel<T, 1024>), dim3(a.n_rows), dim3(1024), 0, st, a);
 }
 
