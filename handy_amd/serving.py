@@ -10,7 +10,8 @@ without waiting; outputs are the caller's buffers, so calls can be captured into
 anything is enqueued."""
 import ctypes as C
 import math
-from typing import NamedTuple, Optional
+import struct
+from typing import Optional
 
 import numpy as np
 
@@ -90,14 +91,23 @@ def _contiguous(shape):
     return tuple(reversed(out))
 
 
+_ATTN = struct.Struct("@5P5q7if")         # wmi_paged_attn (packing bytes takes half the time of filling the ctypes structure)
+assert _ATTN.size == C.sizeof(wr.wmi_paged_attn)
+_NAMES = {}         # dtype object -> name ("float16" and torch.float16 alike)
+
+
 def _dtype(x) -> str:
     d = x.dtype
-    return d if type(d) is str else str(d).replace("torch.", "")
+    n = _NAMES.get(d)
+    if n is None:
+        n = _NAMES[d] = str(d).replace("torch.", "")
+    return n
 
 
 def _flat(x, dtype: str, n: int, name: str):
-    """pointer of a contiguous 1-d array of at least n elements"""
-    if _dtype(x) != dtype or len(x.shape) != 1 or x.shape[0] < n or (n > 1 and x.stride()[0] != 1):
+    """pointer of a contiguous 1-d array of at least n elements (none of no elements)"""
+    s = x.shape
+    if len(s) != 1 or s[0] < n or _dtype(x) != dtype or (n > 1 and x.stride()[0] != 1):
         raise ValueError(f"{name}: expected a contiguous {dtype} array of {n}")
     return x.data_ptr() if n else None
 
@@ -105,9 +115,22 @@ def _flat(x, dtype: str, n: int, name: str):
 def _rows(x, shape, dtype: str, name: str):
     """pointer and the two outer strides of a [rows][heads][dim] array with contiguous heads"""
     st = x.stride()
-    if _dtype(x) != dtype or tuple(x.shape) != shape or (shape[2] > 1 and st[2] != 1):
-        raise ValueError(f"{name}: expected {dtype} {shape} with contiguous last axis")
+    if x.shape != shape or _dtype(x) != dtype or (st[2] != 1 and shape[2] > 1):
+        raise ValueError(f"{name}: expected {dtype} {tuple(shape)} with contiguous last axis")
     return x.data_ptr(), st[0], st[1]
+
+
+def _table(x, n_seq: int):
+    """pointer, row stride and columns of an int32 [n_seq][cols] array with contiguous rows"""
+    s, st = x.shape, x.stride()
+    if len(s) != 2 or s[0] != n_seq or _dtype(x) != "int32" or (st[1] != 1 and s[1] > 1):
+        raise ValueError("block_table: expected int32 [n_seq, cols] with contiguous rows")
+    cols = s[1]
+    return x.data_ptr() if n_seq and cols else None, max(st[0], cols), cols
+
+
+def _lib():
+    return wr._lib or wr.load_library()
 
 
 def _check(rc: int, what: str):
@@ -135,13 +158,18 @@ class PagedCache:
         self.ref = C.byref(self.c)
 
 
-class PagePlan(NamedTuple):
-    """Buffers of one step's plan, int32: cu_q[n_seq + 1], kv_lens[n_seq], slots[rows], positions[rows], counts[4]."""
-    cu_q: object
-    kv_lens: object
-    slots: object
-    positions: object
-    counts: object
+class PagePlan:
+    """Buffers of one step's plan, int32: cu_q[n_seq + 1], kv_lens[n_seq], slots[rows], positions[rows], counts[4]. Keeps the arrays."""
+    __slots__ = ("cu_q", "kv_lens", "slots", "positions", "counts", "n_seq", "n_rows", "_p")
+
+    def __init__(self, cu_q, kv_lens, slots, positions, counts):
+        self.cu_q, self.kv_lens, self.slots, self.positions, self.counts = cu_q, kv_lens, slots, positions, counts
+        self.n_seq, self.n_rows = int(kv_lens.shape[0]), int(slots.shape[0])
+        self._p = (_flat(cu_q, "int32", self.n_seq + 1, "cu_q"), _flat(kv_lens, "int32", self.n_seq, "kv_lens"), _flat(slots, "int32", self.n_rows, "slots"),
+                   _flat(positions, "int32", self.n_rows, "positions"), self.n_rows, _flat(counts, "int32", 4, "counts"))
+
+    def __iter__(self):
+        return iter((self.cu_q, self.kv_lens, self.slots, self.positions, self.counts))
 
     @classmethod
     def allocate(cls, n_seq: int, n_rows: int):
@@ -151,15 +179,12 @@ class PagePlan(NamedTuple):
 def plan_pages(ctx_lens, new_lens, free_pages, block_table, page_tokens: int, out: PagePlan, stream: int = 0) -> PagePlan:
     """Admit requests in order, give them fresh pages from the front of free_pages (entered in block_table[n_seq, cols]) and number
     their rows: see wmi_paged_plan in include/wmi.h. The number of rows planned for is the length of out.slots."""
-    n_seq, cap = int(ctx_lens.shape[0]), int(out.slots.shape[0])
-    if _dtype(block_table) != "int32" or len(block_table.shape) != 2 or block_table.shape[0] != n_seq or (block_table.shape[1] > 1 and block_table.stride()[1] != 1):
-        raise ValueError("block_table: expected int32 [n_seq, cols] with contiguous rows")
-    cols, n_free = int(block_table.shape[1]), int(free_pages.shape[0])
-    rc = wr.load_library().wmi_paged_plan(
-        _flat(ctx_lens, "int32", n_seq, "ctx_lens"), _flat(new_lens, "int32", n_seq, "new_lens"), n_seq, _flat(free_pages, "int32", n_free, "free_pages"), n_free,
-        page_tokens, block_table.data_ptr() if n_seq and cols else None, cols, max(block_table.stride()[0], cols), _flat(out.cu_q, "int32", n_seq + 1, "cu_q"),
-        _flat(out.kv_lens, "int32", n_seq, "kv_lens"), _flat(out.slots, "int32", cap, "slots"), _flat(out.positions, "int32", cap, "positions"), cap,
-        _flat(out.counts, "int32", 4, "counts"), stream)
+    n_seq, n_free = out.n_seq, free_pages.shape[0]
+    tp, stride, cols = _table(block_table, n_seq)
+    if ctx_lens.shape[0] != n_seq or new_lens.shape[0] != n_seq:
+        raise ValueError(f"ctx_lens, new_lens: expected the plan's {n_seq} requests")
+    rc = _lib().wmi_paged_plan(_flat(ctx_lens, "int32", n_seq, "ctx_lens"), _flat(new_lens, "int32", n_seq, "new_lens"), n_seq,
+                               _flat(free_pages, "int32", n_free, "free_pages"), n_free, page_tokens, tp, cols, stride, *out._p, stream)
     if rc:
         _check(rc, "plan_pages")
     return out
@@ -168,11 +193,11 @@ def plan_pages(ctx_lens, new_lens, free_pages, block_table, page_tokens: int, ou
 def write_kv(cache: PagedCache, k_new, v_new, slots, stream: int = 0) -> None:
     """cache[slots[r]] = k_new[r], v_new[r] (rows [n_kv_heads, head_dim], any row and head strides); rows with a slot outside the cache
     are skipped. The slots of one call must be distinct."""
-    n = int(k_new.shape[0])
+    n = k_new.shape[0]
     shape = (n, cache.n_kv_heads, cache.head_dim)
     kp, kr, kh = _rows(k_new, shape, cache.dtype, "k_new")
     vp, vr, vh = _rows(v_new, shape, cache.dtype, "v_new")
-    rc = wr.load_library().wmi_paged_write(cache.ref, kp if n else None, kr, kh, vp if n else None, vr, vh, _flat(slots, "int32", n, "slots"), n, stream)
+    rc = _lib().wmi_paged_write(cache.ref, kp if n else None, kr, kh, vp if n else None, vr, vh, _flat(slots, "int32", n, "slots"), n, stream)
     if rc:
         _check(rc, "write_kv")
 
@@ -180,7 +205,7 @@ def write_kv(cache: PagedCache, k_new, v_new, slots, stream: int = 0) -> None:
 def paged_attention_workspace(cache: PagedCache, n_rows: int, n_q_heads: int, n_seq: int, max_new: int = 0, max_kv: int = 0) -> int:
     """Bytes of device memory `paged_attention` needs for these sizes (0: none)."""
     a = wr.wmi_paged_attn(None, None, None, None, None, 0, 0, 0, 0, 0, 0, n_rows, n_seq, n_q_heads, 0, max_new, max_kv, 1.0)
-    need = wr.load_library().wmi_paged_attention_workspace(cache.ref, C.byref(a))
+    need = _lib().wmi_paged_attention_workspace(cache.ref, C.byref(a))
     if need < 0:
         _check(int(need), "paged_attention_workspace")
     return int(need)
@@ -192,24 +217,20 @@ def paged_attention(q, cache: PagedCache, block_table, cu_q, kv_lens, max_new: i
     > 0 over the last `window` keys only: see wmi_paged_attention in include/wmi.h. max_new / max_kv: the longest request's new and
     total tokens (0: not known; they steer the split of the work). workspace: uint8 device array of `paged_attention_workspace`
     bytes, one for each call that may run at the same time. Returns out."""
-    shape = tuple(q.shape)
-    if len(shape) != 3 or shape[2] != cache.head_dim:
+    shape, dim = q.shape, cache.head_dim
+    if len(shape) != 3 or shape[2] != dim:
         raise ValueError("q: expected [n_rows, n_q_heads, head_dim]")
     qp, qr, qh = _rows(q, shape, cache.dtype, "q")
     op, orow, oh = _rows(out, shape, cache.dtype, "out")
-    n_seq = int(kv_lens.shape[0])
-    bt = block_table
-    if _dtype(bt) != "int32" or len(bt.shape) != 2 or bt.shape[0] != n_seq or (bt.shape[1] > 1 and bt.stride()[1] != 1):
-        raise ValueError("block_table: expected int32 [n_seq, cols] with contiguous rows")
-    cols = int(bt.shape[1])
-    a = wr.wmi_paged_attn(qp, op, bt.data_ptr() if cols else None, _flat(cu_q, "int32", n_seq + 1, "cu_q"), _flat(kv_lens, "int32", n_seq, "kv_lens"), qr, qh, orow, oh,
-                          max(bt.stride()[0], cols), cols, shape[0], n_seq, shape[1], window, max_new, max_kv, cache.head_dim ** -0.5 if scale is None else scale)
+    n_seq = kv_lens.shape[0]
+    tp, stride, cols = _table(block_table, n_seq)
+    a = _ATTN.pack(qp or 0, op or 0, tp or 0, _flat(cu_q, "int32", n_seq + 1, "cu_q") or 0, _flat(kv_lens, "int32", n_seq, "kv_lens") or 0, qr, qh, orow, oh, stride, cols,
+                   shape[0], n_seq, shape[1], window, max_new, max_kv, dim ** -0.5 if scale is None else scale)
     ws, ws_bytes = None, 0
     if workspace is not None:
-        if _dtype(workspace) != "uint8":
-            raise ValueError("workspace: expected a uint8 array")
-        ws, ws_bytes = workspace.data_ptr(), workspace.numel()
-    rc = wr.load_library().wmi_paged_attention(cache.ref, C.byref(a), ws, ws_bytes, stream)
+        ws_bytes = workspace.shape[0]
+        ws = _flat(workspace, "uint8", ws_bytes, "workspace")
+    rc = _lib().wmi_paged_attention(cache.ref, a, ws, ws_bytes, stream)
     if rc:
         _check(rc, "paged_attention")
     return out
@@ -219,15 +240,15 @@ def sample_tokens(logits, uniform, token, logprob=None, temperature=None, top_k=
     """One token a row of logits [n_rows, n_vocab] (float32, float16 or bfloat16) into token (int32), from uniform numbers in [0, 1) (float32,
     one a row): see wmi_sample_tokens in include/wmi.h. temperature, top_p, min_p (float32) and top_k (int32) are per row or None.
     logprob (float32, may be None): the token's log-probability before the filters. Returns token."""
-    dt = _dtype(logits)
-    if dt not in _DTYPES or len(logits.shape) != 2 or (logits.shape[1] > 1 and logits.stride()[1] != 1):
+    dt, shape, st = _DTYPES.get(_dtype(logits), -1), logits.shape, logits.stride()
+    if dt < 0 or len(shape) != 2 or (st[1] != 1 and shape[1] > 1):
         raise ValueError("logits: expected float32, float16 or bfloat16 [n_rows, n_vocab] with contiguous rows")
-    n, v = int(logits.shape[0]), int(logits.shape[1])
-    opt = lambda x, d, name: None if x is None else _flat(x, d, n, name)
-    rc = wr.load_library().wmi_sample_tokens(
-        logits.data_ptr() if n else None, _DTYPES[dt], logits.stride()[0], n, v, _flat(uniform, "float32", n, "uniform"), opt(temperature, "float32", "temperature"),
-        opt(top_k, "int32", "top_k"), opt(top_p, "float32", "top_p"), opt(min_p, "float32", "min_p"), _flat(token, "int32", n, "token"),
-        opt(logprob, "float32", "logprob"), stream)
+    n, v = shape
+    rc = _lib().wmi_sample_tokens(
+        logits.data_ptr() if n else None, dt, st[0], n, v, _flat(uniform, "float32", n, "uniform"),
+        None if temperature is None else _flat(temperature, "float32", n, "temperature"), None if top_k is None else _flat(top_k, "int32", n, "top_k"),
+        None if top_p is None else _flat(top_p, "float32", n, "top_p"), None if min_p is None else _flat(min_p, "float32", n, "min_p"),
+        _flat(token, "int32", n, "token"), None if logprob is None else _flat(logprob, "float32", n, "logprob"), stream)
     if rc:
         _check(rc, "sample_tokens")
     return token

@@ -265,7 +265,7 @@ def load_library(path: Optional[str] = None):
     L.wmi_dev_stream_create.restype = vp; L.wmi_dev_stream_create.argtypes = []
     L.wmi_dev_stream_sync.restype = ci; L.wmi_dev_stream_sync.argtypes = [vp]
     L.wmi_dev_stream_destroy.restype = None; L.wmi_dev_stream_destroy.argtypes = [vp]
-    cache_p, attn_p = C.POINTER(wmi_paged_cache), C.POINTER(wmi_paged_attn)
+    cache_p, attn_p = C.POINTER(wmi_paged_cache), vp          # (a wmi_paged_attn by reference, or its bytes)
     L.wmi_paged_plan.restype = ci; L.wmi_paged_plan.argtypes = [vp, vp, ci, vp, ci, ci, vp, ci, ll, vp, vp, vp, vp, ci, vp, vp]
     L.wmi_paged_write.restype = ci; L.wmi_paged_write.argtypes = [cache_p, vp, ll, ll, vp, ll, ll, vp, ci, vp]
     L.wmi_paged_attention_workspace.restype = ll; L.wmi_paged_attention_workspace.argtypes = [cache_p, attn_p]

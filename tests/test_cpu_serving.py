@@ -108,10 +108,13 @@ def test_python_layer_refuses_wrong_shapes_and_types():
         with pytest.raises(ValueError):
             sv.write_kv(cache, *a)
     plan = sv.PagePlan(i32(4), i32(3), i32(9), i32(9), i32(4))
-    for a in ((i32(3), i32(2), i32(5), i32(3, 4), plan), (i32(3), i32(3), i32(5), i32(2, 4), plan), (i32(3), i32(3), Fake((5,), "int64"), i32(3, 4), plan),
-              (i32(3), i32(3), i32(5), i32(3, 4), plan._replace(cu_q=i32(3))), (i32(3), i32(3), i32(5), i32(3, 4), plan._replace(positions=i32(8)))):
+    for a in ((i32(3), i32(2), i32(5), i32(3, 4)), (i32(4), i32(3), i32(5), i32(3, 4)), (i32(3), i32(3), i32(5), i32(2, 4)), (i32(3), i32(3), Fake((5,), "int64"), i32(3, 4)),
+              (i32(3), i32(3), i32(5), Fake((3, 4), "int32", (8, 2)))):
         with pytest.raises(ValueError):
-            sv.plan_pages(a[0], a[1], a[2], a[3], 16, a[4])
+            sv.plan_pages(*a, 16, plan)
+    for bad in ((i32(3), i32(3), i32(9), i32(9), i32(4)), (i32(4), i32(3), i32(9), i32(8), i32(4)), (i32(4), i32(3), i32(9), i32(9), i32(3)), (Fake((4,), "int64"), i32(3), i32(9), i32(9), i32(4))):
+        with pytest.raises(ValueError):
+            sv.PagePlan(*bad)
     x, u, t = Fake((2, 50), "float32"), Fake((2,), "float32"), i32(2)
     for a, kw in (((Fake((2, 50), "float64"), u, t), {}), ((Fake((100,), "float32"), u, t), {}), ((x, Fake((1,), "float32"), t), {}), ((x, u, Fake((2,), "int64")), {}),
                   ((x, u, t), dict(top_k=Fake((2,), "float32"))), ((x, u, t), dict(temperature=i32(2))), ((x, u, t), dict(logprob=Fake((2,), "float16"))),
