@@ -206,6 +206,7 @@ __device__ __forceinline__ int attn_parts(int n_kt, int splits, int least) { ret
 
 constexpr int kStepRows = 16, kStepKeys = 16, kChunkRows = 128, kChunkKeys = 64;
 constexpr int kStepLeast = 32, kChunkLeast = 4;        // shortest part, in key tiles (512 and 256 keys): below that the join costs more than it saves
+constexpr int kMaxParts = 256;                         // the join gives every part a thread
 constexpr float kMoveBy = 8.0f;
 
 // partial results of a split call: [part][row][query head][DP] accumulators, then {reference exponent, sum}
@@ -241,6 +242,13 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(PagedAttn a, AttnPar
     const T *kc = (const T *)a.k + head * a.head_stride, *vc = (const T *)a.v + head * a.head_stride;
     char *mine = smem + wave * 4 * TILE;
     const int lrow = lane / CH, lslot = lane % CH;
+    const long v_minus_k = (const char *)vc - (const char *)kc;
+    const T *kl[NI];                                                       // a lane's address in load i of a tile, from the tile's first key on
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        const int ch = lslot ^ swz<DP>(i * RPI + lrow);
+        kl[i] = kc + (i * RPI + lrow) * a.token_stride + (ch * 8 < a.dim ? ch * 8 : 0);         // (dims past the head's: any of the key's own, q is 0 there)
+    }
 
     for (int r0 = 0; r0 < rows; r0 += kStepRows) {
         const int r1 = min(rows, r0 + kStepRows);
@@ -281,17 +289,28 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(PagedAttn a, AttnPar
             }
         };
         auto page_ok = [&](int p) { return (unsigned)p < (unsigned)a.n_pages; };
+        auto copy = [&](const T *k, const T *v, int buf, int i) __attribute__((always_inline)) {       // (non-temporal: every byte is read once in the call)
+            char *kd = mine + buf * 2 * TILE + i * 1024;
+            __builtin_amdgcn_global_load_lds((const WMI_GLB void *)k, (WMI_LDS void *)kd, 16, 0, 2);
+            __builtin_amdgcn_global_load_lds((const WMI_GLB void *)v, (WMI_LDS void *)(kd + TILE), 16, 0, 2);
+        };
         auto stage = [&](int t, int buf, int at) {
-            char *kd = mine + buf * 2 * TILE;
-            const int up = PAGE16 ? __builtin_amdgcn_readlane(pg[0], at) : 0;
+            const int k0 = t * kStepKeys, up = PAGE16 ? __builtin_amdgcn_readlane(pg[0], at) : 0;
+            if (PAGE16 && k0 >= lo && k0 + kStepKeys <= hi && page_ok(up)) {             // all keys exist, in one page: a scalar plus a constant of the lane
+                const long off = up * a.page_stride + (long)(k0 & ((1 << a.lp) - 1)) * a.token_stride;
+#pragma unroll
+                for (int i = 0; i < NI; i++) {
+                    const T *k = kl[i] + off;
+                    copy(k, (const T *)((const char *)k + v_minus_k), buf, i);
+                }
+                return;
+            }
 #pragma unroll
             for (int i = 0; i < NI; i++) {
-                const int lr = i * RPI + lrow, j = t * kStepKeys + lr, ch = lslot ^ swz<DP>(lr), page = PAGE16 ? up : pg[i];
+                const int lr = i * RPI + lrow, j = k0 + lr, ch = lslot ^ swz<DP>(lr), page = PAGE16 ? up : pg[i];
                 const bool on = j >= lo && j < hi && page_ok(page) && ch * 8 < a.dim;
                 const long off = page * a.page_stride + (long)(j & ((1 << a.lp) - 1)) * a.token_stride + ch * 8;
-                const T *ksrc = on ? kc + off : (const T *)attn_zero_chunk, *vsrc = on ? vc + off : (const T *)attn_zero_chunk;
-                __builtin_amdgcn_global_load_lds((const WMI_GLB void *)ksrc, (WMI_LDS void *)(kd + i * 1024), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const WMI_GLB void *)vsrc, (WMI_LDS void *)(kd + TILE + i * 1024), 16, 0, 0);
+                copy(on ? kc + off : (const T *)attn_zero_chunk, on ? vc + off : (const T *)attn_zero_chunk, buf, i);
             }
         };
         auto compute = [&](int t, int buf, bool page_bad, unsigned bad_keys) {
@@ -487,32 +506,54 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a, AttnPa
         if (a.scale < 0.0f) x ^= M::kSign;
         qf[ks] = __builtin_bit_cast(V8, x);
     }
-    const int lrow = lane / CH, lslot = lane % CH;
-    int pg[NI];
-    auto entries = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < NI; i++) { const int j = t * kChunkKeys + (wave + 4 * i) * RPI + lrow; pg[i] = j >= lo && j < hi ? tbl[j >> a.lp] : 0; }
+    // Loads: one wave instruction moves RPI keys (1 KB) of K or V; this wave's are key groups wave, wave + 4, .. of a tile. Where a
+    // group lies in one page and every key of the tile exists, its address is a scalar (page, token) plus a constant of the lane;
+    // the chunk a lane fetches does not depend on which of the wave's groups it is.
+    const int lrow = lane / CH, lslot = lane % CH, lch = lslot ^ swz<DP>(wave * RPI + lrow), dch = lch * 8 < a.dim ? lch * 8 : 0;
+    const T *kl = kc + lrow * a.token_stride + dch;                        // (dims past the head's: any of the key's own, q is 0 there)
+    const long v_minus_k = (const char *)vc - (const char *)kc;
+    int pages;                                                             // lane l: page of key group l of the next tile
+    auto entries = [&](int t) { const int j = t * kChunkKeys + (lane & (kChunkKeys / RPI - 1)) * RPI; pages = tbl[min(max(j, lo), hi - 1) >> a.lp]; };
+    auto copy = [&](const T *k, const T *v, int buf, int i) __attribute__((always_inline)) {
+        char *dst = smem + buf * 2 * TILE + (wave + 4 * i) * 1024;
+        __builtin_amdgcn_global_load_lds((const WMI_GLB void *)k, (WMI_LDS void *)dst, 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((const WMI_GLB void *)v, (WMI_LDS void *)(dst + TILE), 16, 0, 0);
     };
     auto stage = [&](int t, int buf) {
-        char *kd = smem + buf * 2 * TILE;
-        bool bad = false;
+        const int k0 = t * kChunkKeys;
+        bool inner = k0 >= lo && k0 + kChunkKeys <= hi && (1 << a.lp) >= RPI;
+        if (inner) {
 #pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const int lr = (wave + 4 * i) * RPI + lrow, j = t * kChunkKeys + lr, ch = lslot ^ swz<DP>(lr);
-            const bool has = (unsigned)pg[i] < (unsigned)a.n_pages, on = j >= lo && j < hi && has && ch * 8 < a.dim;
-            bad |= !has;
-            const long off = pg[i] * a.page_stride + (long)(j & ((1 << a.lp) - 1)) * a.token_stride + ch * 8;
-            const T *ksrc = on ? kc + off : (const T *)attn_zero_chunk, *vsrc = on ? vc + off : (const T *)attn_zero_chunk;
-            char *dst = kd + (wave + 4 * i) * 1024;
-            __builtin_amdgcn_global_load_lds((const WMI_GLB void *)ksrc, (WMI_LDS void *)dst, 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((const WMI_GLB void *)vsrc, (WMI_LDS void *)(dst + TILE), 16, 0, 0);
+            for (int i = 0; i < NI; i++) inner &= (unsigned)__builtin_amdgcn_readlane(pages, wave + 4 * i) < (unsigned)a.n_pages;
         }
-        const bool any = __any(bad);
+        bool any = false;
+        if (inner) {
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int page = __builtin_amdgcn_readlane(pages, wave + 4 * i), token = (k0 + (wave + 4 * i) * RPI) & ((1 << a.lp) - 1);
+                const T *k = kl + (page * a.page_stride + token * a.token_stride);
+                copy(k, (const T *)((const char *)k + v_minus_k), buf, i);
+            }
+        } else {                                                           // a tile at an end of the keys, or with a page that is not there
+            bool bad = false;
+            int pg[NI];
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int j = k0 + (wave + 4 * i) * RPI + lrow;
+                const bool in = j >= lo && j < hi;
+                pg[i] = tbl[min(max(j, lo), hi - 1) >> a.lp];
+                const bool has = (unsigned)pg[i] < (unsigned)a.n_pages, on = in && has && lch * 8 < a.dim;
+                bad |= in && !has;
+                const long off = pg[i] * a.page_stride + (long)(j & ((1 << a.lp) - 1)) * a.token_stride + lch * 8;
+                copy(on ? kc + off : (const T *)attn_zero_chunk, on ? vc + off : (const T *)attn_zero_chunk, buf, i);
+            }
+            any = __any(bad);
+            if (any && lslot == 0) {
+#pragma unroll
+                for (int i = 0; i < NI; i++) bad_key[buf][(wave + 4 * i) * RPI + lrow] = (unsigned)pg[i] >= (unsigned)a.n_pages;
+            }
+        }
         if (lane == 0) bad_flag[buf][wave] = any;
-        if (any && lslot == 0) {
-#pragma unroll
-            for (int i = 0; i < NI; i++) bad_key[buf][(wave + 4 * i) * RPI + lrow] = (unsigned)pg[i] >= (unsigned)a.n_pages;
-        }
     };
     f32x16 o[NB];
 #pragma unroll
@@ -644,14 +685,13 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a, AttnPa
     }
 }
 
-// out = sum over a row's parts, in their order. One wave a (row, query head); the number of parts follows from the lengths as in the
-// kernel that made them (tiles of ROWS packed rows, KEYS keys).
+// out = sum over a row's parts. One workgroup a (row, query head), the parts dealt to its 4 waves and added up in a fixed order; the
+// number of parts follows from the lengths as in the kernel that made them (tiles of ROWS packed rows, KEYS keys).
 template <class T, int DP, int ROWS, int KEYS, int LEAST>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, AttnParts ps) {
-    const int lane = threadIdx.x & 63, hqs = a.hkv * a.group;
-    const long id = blockIdx.x * 4L + (threadIdx.x >> 6);
-    const int row = (int)(id / hqs), hq = (int)(id % hqs);
-    if (row >= a.n_rows) return;
+    constexpr int E = DP / 64;                                             // dims of a lane
+    __shared__ float scale_of[kMaxParts], red[4][DP], sum[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hqs = a.hkv * a.group, row = blockIdx.x / hqs, hq = blockIdx.x % hqs;
     int lo = 0, hi = a.n_seq;
     while (lo < hi) { const int x = (lo + hi) >> 1; if (a.cu[x + 1] <= row) lo = x + 1; else hi = x; }
     if (lo >= a.n_seq || row < a.cu[lo]) return;
@@ -662,19 +702,30 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, AttnParts 
     const int n_kt = max((k1 + KEYS - 1) / KEYS - k0 / KEYS, 0), parts = attn_parts(n_kt, ps.splits, LEAST);
     if (parts == 1) return;                                                // written by the kernel itself
     const long stride = (long)a.n_rows * hqs, at = (long)row * hqs + hq;
-    float m = -INFINITY, l = 0.0f, acc0 = 0.0f, acc1 = 0.0f;
-    for (int p = 0; p < parts; p++) m = fmaxf(m, ps.ml[p * stride + at].x);
-    for (int p = 0; p < parts; p++) {
-        const float2 ml = ps.ml[p * stride + at];
-        const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
-        l += ml.y * f;
-        const float *src = ps.o + (p * stride + at) * DP + lane * (DP / 64);
-        acc0 += src[0] * f;
-        if (DP == 128) acc1 += src[1] * f;
+    const float2 ml = tid < parts ? ps.ml[tid * stride + at] : make_float2(-INFINITY, 0.0f);
+    float m = ml.x;
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if (lane == 0) sum[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(sum[0], sum[1]), fmaxf(sum[2], sum[3]));
+    const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
+    float l = ml.y * f;
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+    scale_of[tid] = f;
+    __syncthreads();
+    if (lane == 0) sum[wave] = l;
+    float acc[E] = {};
+    const float *src = ps.o + at * DP + lane * E;
+#pragma unroll 8
+    for (int p = wave; p < parts; p += 4) {
+#pragma unroll
+        for (int e = 0; e < E; e++) acc[e] += src[p * stride * DP + e] * scale_of[p];
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T *dst = (T *)a.out + row * a.o_row + hq * a.o_head + lane * (DP / 64);
-    if (lane * (DP / 64) < a.dim) { dst[0] = (T)(acc0 * inv); if (DP == 128) dst[1] = (T)(acc1 * inv); }
+#pragma unroll
+    for (int e = 0; e < E; e++) red[wave][lane * E + e] = acc[e];
+    __syncthreads();
+    l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    if (tid < a.dim) ((T *)a.out)[row * a.o_row + hq * a.o_head + tid] = (T)(((red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid])) * (l == 0.0f ? 0.0f : 1.0f / l));
 }
 
 // How a call is cut up. The step kernel takes calls whose requests bring at most 16 packed rows each, as far as the caller says;
@@ -686,9 +737,9 @@ static AttnShape attn_shape(const PagedAttn &a) {
     s.step = new_rows <= kStepRows;
     s.tiles = s.step ? a.n_seq : (int)((long)a.n_rows * a.group / kChunkRows + a.n_seq);
     const long work = (long)s.tiles * a.hkv, full = s.step ? 2048 : 1024, least = s.step ? kStepLeast * kStepKeys : kChunkLeast * kChunkKeys;
-    long n = (full + work - 1) / work;
+    long n = full / work;
     if (n > keys / least) n = keys / least;
-    s.splits = n < 1 ? 1 : n > 256 ? 256 : (int)n;
+    s.splits = n < 1 ? 1 : n > kMaxParts ? kMaxParts : (int)n;
     return s;
 }
 
@@ -703,7 +754,7 @@ template <class T, int DP> static bool attn_launch(const PagedAttn &a, void *wor
     const AttnShape s = attn_shape(a);
     const long pairs = (long)a.n_rows * a.hkv * a.group;
     const AttnParts ps{(float *)workspace, (float2 *)((float *)workspace + (s.splits == 1 ? 0 : s.splits * pairs * DP)), s.splits};
-    const unsigned join = (unsigned)((pairs + 3) / 4);
+    const unsigned join = (unsigned)pairs;
     if (s.step) {
         const dim3 grid((unsigned)(a.n_seq * a.hkv), s.splits);
         if (a.lp >= 4) hipLaunchKernelGGL((paged_step_kernel<T, DP, true>), grid, dim3(256), 0, st, a, ps);
