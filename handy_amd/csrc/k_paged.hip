@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
 // The query rows of a request's tokens and of the heads that share a key head are packed into one list, row r = token * group +
 // head, so that every K and V byte is read once for all of them.
 //   paged_step_kernel    up to 16 packed rows (single tokens): bound by HBM. Each wave streams its own 16-key tiles.
-//   paged_chunk_kernel   128 packed rows a workgroup, 64-key tiles shared by its waves: bound by MFMA issue and LDS reads.
+//   paged_chunk_kernel   128 or 256 packed rows a workgroup, 64-key tiles shared by its waves.
 // The keys of a tile of rows may be split over workgroups; paged_join_kernel adds the parts up.
 // The reference exponent of a row moves only when a score passes it by more than 8 (in powers of two): probabilities stay below
 // 2^8, which both 16-bit types hold at full relative precision, and the accumulators are rescaled rarely instead of every tile.
@@ -204,7 +204,7 @@ __device__ __forceinline__ void attn_keys(const PagedAttn &a, const AttnReq &q, 
 // how many parts the keys of a tile of rows are cut into: at most `splits`, none shorter than `least` key tiles
 __device__ __forceinline__ int attn_parts(int n_kt, int splits, int least) { return max(1, min(splits, n_kt / least)); }
 
-constexpr int kStepRows = 16, kStepKeys = 16, kChunkRows = 128, kChunkKeys = 64;
+constexpr int kStepRows = 16, kStepKeys = 16, kChunkKeys = 64;
 constexpr int kStepLeast = 32, kChunkLeast = 4;        // shortest part, in key tiles (512 and 256 keys): below that the join costs more than it saves
 constexpr int kMaxParts = 256;                         // the join gives every part a thread
 constexpr float kMoveBy = 8.0f;
@@ -452,20 +452,20 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(PagedAttn a, AttnPar
 }
 
 // ---- chunks of new tokens
-// One workgroup = 128 packed rows of a request (32 a wave), one key head, one part of the keys. A row tile is found from the
-// workgroup's number alone: request i's tiles start at number floor(cu[i] * group / 128) + i, which leaves room for all of them
+// One workgroup = 4 or 8 waves of 32 packed rows of a request, one key head, one part of the keys. A row tile is found from the
+// workgroup's number alone: request i's tiles start at number floor(cu[i] * group / rows) + i, which leaves room for all of them
 // (a few numbers stay empty). Workgroups are dealt round-robin to the 8 XCDs: every XCD gets a contiguous run of (head, row
 // tile), so that the row tiles that stream the same keys share an L2, the ones with the most keys first.
 // Keys a row sees and others of its tile do not are masked to -infinity, p = 0; what V holds there must not be infinite or NaN in
 // the product, so in tiles that need a mask such values are taken out and reach only the rows that do see them (as NaN).
-template <class T, int DP>
-__global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a, AttnParts ps, int n_tiles) {
+template <class T, int DP, int WV>
+__global__ __launch_bounds__(64 * WV, 2) void paged_chunk_kernel(PagedAttn a, AttnParts ps, int n_tiles) {
     typedef Mma<T> M;
     typedef typename M::V8 V8;
     typedef typename M::V4 V4;
-    constexpr int CH = DP / 8, RPI = 64 / CH, NI = kChunkKeys / RPI / 4, TILE = kChunkKeys * DP * 2, NB = DP / 32, NK = DP / 16;
+    constexpr int ROWS = 32 * WV, CH = DP / 8, RPI = 64 / CH, NI = kChunkKeys / RPI / WV, TILE = kChunkKeys * DP * 2, NB = DP / 32, NK = DP / 16;
     __shared__ __attribute__((aligned(16))) char smem[2 * 2 * TILE];
-    __shared__ __attribute__((aligned(16))) unsigned bad_flag[2][4];       // per buffer: some key of this wave's share has no page ...
+    __shared__ __attribute__((aligned(16))) unsigned bad_flag[2][WV];       // per buffer: some key of this wave's share has no page ...
     __shared__ unsigned char bad_key[2][kChunkKeys];                       // ... and which
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n32 = lane & 31, h = lane >> 5;
     const int nblk = gridDim.x, xq = nblk >> 3, xr = nblk & 7, xcd = blockIdx.x & 7, xi = blockIdx.x >> 3;
@@ -474,16 +474,16 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a, AttnPa
     int req = 0;
     for (int left = a.n_seq; left > 1;) {                                  // the last request whose first tile number is <= tile, 64 ways at a time
         const int step = (left + 63) / 64, i = req + lane * step;
-        const bool ok = lane * step < left && (long)a.cu[i] * a.group / kChunkRows + i <= tile;
+        const bool ok = lane * step < left && (long)a.cu[i] * a.group / ROWS + i <= tile;
         const int k = max(__popcll(__ballot(ok)) - 1, 0);
         req += k * step; left = min(step, left - k * step);
     }
     req = __builtin_amdgcn_readfirstlane(req);
     const AttnReq rq = attn_req(a, req);
-    const long r0l = ((long)tile - ((long)a.cu[req] * a.group / kChunkRows + req)) * kChunkRows;
+    const long r0l = ((long)tile - ((long)a.cu[req] * a.group / ROWS + req)) * ROWS;
     const int rows = rq.n * a.group;
     if (r0l < 0 || r0l >= rows) return;
-    const int r0 = (int)r0l, r1 = min(rows, r0 + kChunkRows);
+    const int r0 = (int)r0l, r1 = min(rows, r0 + ROWS);
     int lo, hi;
     attn_keys(a, rq, r0, r1, lo, hi);
     const int kt0 = lo / kChunkKeys, n_kt = max((hi + kChunkKeys - 1) / kChunkKeys - kt0, 0), parts = attn_parts(n_kt, ps.splits, kChunkLeast);
@@ -506,16 +506,16 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a, AttnPa
         if (a.scale < 0.0f) x ^= M::kSign;
         qf[ks] = __builtin_bit_cast(V8, x);
     }
-    // Loads: one wave instruction moves RPI keys (1 KB) of K or V; this wave's are key groups wave, wave + 4, .. of a tile. Where a
+    // Loads: one wave instruction moves RPI keys (1 KB) of K or V; this wave's are key groups wave, wave + WV, .. of a tile. Where a
     // group lies in one page and every key of the tile exists, its address is a scalar (page, token) plus a constant of the lane;
     // the chunk a lane fetches does not depend on which of the wave's groups it is.
     const int lrow = lane / CH, lslot = lane % CH, lch = lslot ^ swz<DP>(wave * RPI + lrow), dch = lch * 8 < a.dim ? lch * 8 : 0;
     const T *kl = kc + lrow * a.token_stride + dch;                        // (dims past the head's: any of the key's own, q is 0 there)
     const long v_minus_k = (const char *)vc - (const char *)kc;
-    int pages;                                                             // lane l: page of key group l of the next tile
-    auto entries = [&](int t) { const int j = t * kChunkKeys + (lane & (kChunkKeys / RPI - 1)) * RPI; pages = tbl[min(max(j, lo), hi - 1) >> a.lp]; };
+    int pages;                                                             // lane l: page of key group l of the tile that is loaded next
+    auto entries = [&](int t) { const int j = t * kChunkKeys + (lane & (kChunkKeys / RPI - 1)) * RPI; return tbl[min(max(j, lo), hi - 1) >> a.lp]; };
     auto copy = [&](const T *k, const T *v, int buf, int i) __attribute__((always_inline)) {
-        char *dst = smem + buf * 2 * TILE + (wave + 4 * i) * 1024;
+        char *dst = smem + buf * 2 * TILE + (wave + WV * i) * 1024;
         __builtin_amdgcn_global_load_lds((const WMI_GLB void *)k, (WMI_LDS void *)dst, 16, 0, 0);
         __builtin_amdgcn_global_load_lds((const WMI_GLB void *)v, (WMI_LDS void *)(dst + TILE), 16, 0, 0);
     };
@@ -524,13 +524,13 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a, AttnPa
         bool inner = k0 >= lo && k0 + kChunkKeys <= hi && (1 << a.lp) >= RPI;
         if (inner) {
 #pragma unroll
-            for (int i = 0; i < NI; i++) inner &= (unsigned)__builtin_amdgcn_readlane(pages, wave + 4 * i) < (unsigned)a.n_pages;
+            for (int i = 0; i < NI; i++) inner &= (unsigned)__builtin_amdgcn_readlane(pages, wave + WV * i) < (unsigned)a.n_pages;
         }
         bool any = false;
         if (inner) {
 #pragma unroll
             for (int i = 0; i < NI; i++) {
-                const int page = __builtin_amdgcn_readlane(pages, wave + 4 * i), token = (k0 + (wave + 4 * i) * RPI) & ((1 << a.lp) - 1);
+                const int page = __builtin_amdgcn_readlane(pages, wave + WV * i), token = (k0 + (wave + WV * i) * RPI) & ((1 << a.lp) - 1);
                 const T *k = kl + (page * a.page_stride + token * a.token_stride);
                 copy(k, (const T *)((const char *)k + v_minus_k), buf, i);
             }
@@ -539,7 +539,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a, AttnPa
             int pg[NI];
 #pragma unroll
             for (int i = 0; i < NI; i++) {
-                const int j = k0 + (wave + 4 * i) * RPI + lrow;
+                const int j = k0 + (wave + WV * i) * RPI + lrow;
                 const bool in = j >= lo && j < hi;
                 pg[i] = tbl[min(max(j, lo), hi - 1) >> a.lp];
                 const bool has = (unsigned)pg[i] < (unsigned)a.n_pages, on = in && has && lch * 8 < a.dim;
@@ -550,7 +550,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a, AttnPa
             any = __any(bad);
             if (any && lslot == 0) {
 #pragma unroll
-                for (int i = 0; i < NI; i++) bad_key[buf][(wave + 4 * i) * RPI + lrow] = (unsigned)pg[i] >= (unsigned)a.n_pages;
+                for (int i = 0; i < NI; i++) bad_key[buf][(wave + WV * i) * RPI + lrow] = (unsigned)pg[i] >= (unsigned)a.n_pages;
             }
         }
         if (lane == 0) bad_flag[buf][wave] = any;
@@ -576,11 +576,11 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a, AttnPa
         }
     };
 
-    if (t0 < t1) { entries(t0); stage(t0, 0); entries(t0 + 1); }
+    if (t0 < t1) { pages = entries(t0); stage(t0, 0); pages = entries(t0 + 1); }
     for (int t = t0; t < t1; t++) {
         const int buf = (t - t0) & 1, k0 = t * kChunkKeys;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // everybody's share of this tile has landed, the other buffer is free
-        if (t + 1 < t1) { stage(t + 1, buf ^ 1); entries(t + 2); }
+        if (t + 1 < t1) { stage(t + 1, buf ^ 1); pages = entries(t + 2); }
         if (!busy || k0 > pmax || (a.window > 0 && k0 + kChunkKeys <= pmin - a.window + 1)) continue;
         const char *kb = smem + buf * 2 * TILE, *vb = kb + TILE;
         f32x16 s[2];
@@ -591,8 +591,10 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a, AttnPa
 #pragma unroll
             for (int ks = 0; ks < NK; ks++) s[kh] = M::m32(*(const V8 *)(kb + kh * 32 * DP * 2 + (kf ^ (ks * 32))), qf[ks], s[kh]);
         }
-        const uint4 fl = *(const uint4 *)bad_flag[buf];
-        const bool hole = __builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w) != 0;
+        unsigned flags = 0;
+#pragma unroll
+        for (int w = 0; w < WV; w++) flags |= bad_flag[buf][w];
+        const bool hole = __builtin_amdgcn_readfirstlane(flags) != 0;
         const bool mixed = k0 + kChunkKeys - 1 > pmin || (a.window > 0 && k0 < pmax - a.window + 1) || hole;
         if (mixed) {
 #pragma unroll
@@ -601,7 +603,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a, AttnPa
                 for (int i = 0; i < 16; i++) {
                     const int kk = kh * 32 + (i & 3) + 8 * (i >> 2) + 4 * h, j = k0 + kk;
                     if (j > pos || j < klow) s[kh][i] = -INFINITY;
-                    if (hole && bad_flag[buf][(kk / RPI) & 3] && bad_key[buf][kk]) s[kh][i] = -INFINITY;
+                    if (hole && bad_flag[buf][(kk / RPI) % WV] && bad_key[buf][kk]) s[kh][i] = -INFINITY;
                 }
         }
         float mx = -INFINITY;
@@ -730,12 +732,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, AttnParts 
 
 // How a call is cut up. The step kernel takes calls whose requests bring at most 16 packed rows each, as far as the caller says;
 // it is right for any, 16 rows at a time.
-struct AttnShape { bool step; int tiles, splits; };
+struct AttnShape { bool step; int waves, tiles, splits; };
 static AttnShape attn_shape(const PagedAttn &a) {
     AttnShape s;
     const long new_rows = (long)(a.max_new > 0 ? a.max_new : a.n_rows) * a.group, keys = a.max_kv > 0 ? a.max_kv : 0x7fffffff;
     s.step = new_rows <= kStepRows;
-    s.tiles = s.step ? a.n_seq : (int)((long)a.n_rows * a.group / kChunkRows + a.n_seq);
+    // Eight waves share a tile where the keys of one head outgrow an XCD's 4 MB of L2 (8192 keys of 128 dims) and there are rows for
+    // them: half the tile traffic (chunks of 4096 at 28 000 keys 5.2 ms against 5.65). Four otherwise: less waiting for each
+    // other and less idle in a request's last tile (prompts of up to 224 tokens 34 us against 54, 64 dims 3.1 ms against 3.5).
+    s.waves = a.dim > 64 && keys > 8192 && new_rows >= 256 ? 8 : 4;
+    s.tiles = s.step ? a.n_seq : (int)((long)a.n_rows * a.group / (32 * s.waves) + a.n_seq);
     const long work = (long)s.tiles * a.hkv, full = s.step ? 2048 : 1024, least = s.step ? kStepLeast * kStepKeys : kChunkLeast * kChunkKeys;
     long n = full / work;
     if (n > keys / least) n = keys / least;
@@ -761,8 +767,11 @@ template <class T, int DP> static bool attn_launch(const PagedAttn &a, void *wor
         else hipLaunchKernelGGL((paged_step_kernel<T, DP, false>), grid, dim3(256), 0, st, a, ps);
         if (s.splits > 1) hipLaunchKernelGGL((paged_join_kernel<T, DP, kStepRows, kStepKeys, kStepLeast>), dim3(join), dim3(256), 0, st, a, ps);
     } else {
-        hipLaunchKernelGGL((paged_chunk_kernel<T, DP>), dim3((unsigned)((long)s.tiles * a.hkv * s.splits)), dim3(256), 0, st, a, ps, s.tiles);
-        if (s.splits > 1) hipLaunchKernelGGL((paged_join_kernel<T, DP, kChunkRows, kChunkKeys, kChunkLeast>), dim3(join), dim3(256), 0, st, a, ps);
+        const dim3 grid((unsigned)((long)s.tiles * a.hkv * s.splits)), threads(64 * s.waves);
+        if (s.waves == 8) hipLaunchKernelGGL((paged_chunk_kernel<T, DP, 8>), grid, threads, 0, st, a, ps, s.tiles);
+        else hipLaunchKernelGGL((paged_chunk_kernel<T, DP, 4>), grid, threads, 0, st, a, ps, s.tiles);
+        if (s.splits > 1 && s.waves == 8) hipLaunchKernelGGL((paged_join_kernel<T, DP, 256, kChunkKeys, kChunkLeast>), dim3(join), dim3(256), 0, st, a, ps);
+        else if (s.splits > 1) hipLaunchKernelGGL((paged_join_kernel<T, DP, 128, kChunkKeys, kChunkLeast>), dim3(join), dim3(256), 0, st, a, ps);
     }
     return hipGetLastError() == hipSuccess;
 }
