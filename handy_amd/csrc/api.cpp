@@ -347,6 +347,13 @@ const char *whisper_full_get_token_text(struct whisper_context *c, int i, int j)
 
 // ------------------------------------------------------------------------------------------ wmi extras
 void wmi_set_force_tokens(struct whisper_state *s, int n) { if (Engine *e = ENG(s)) e->force_tokens = n; }
+int wmi_set_device_draws(struct whisper_state *s, int on, int top_k, float top_p, float min_p) {
+    Engine *e = ENG(s);
+    if (!e || top_k < 0 || !(top_p > 0.0f && top_p <= 1.0f) || !(min_p >= 0.0f && min_p <= 1.0f)) return -1;
+    e->device_draws = on != 0; e->draw_top_k = top_k; e->draw_top_p = top_p; e->draw_min_p = min_p;
+    return 0;
+}
+int wmi_set_prompt_attention(struct whisper_state *s, int on) { Engine *e = ENG(s); if (!e) return -1; e->prompt_attention = on != 0; return 0; }
 void wmi_set_beam_candidates_sampled(struct whisper_state *s, int v) { if (Engine *e = ENG(s)) e->beam_sampled = v != 0; }
 int wmi_mel_batch_device(struct whisper_context *, struct whisper_state *s, const float *pcm_dev, const long long *offsets, const int *n, int B) {
     WMI_TRY

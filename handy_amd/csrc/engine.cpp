@@ -135,8 +135,8 @@ bool Engine::alloc_workspaces() {
     lrows_cap_ = round_up(std::max(max_seqs, 8), 256);
     ok &= dxl_.ensure((size_t)lrows_cap_ * d * sizeof(f16));
     ok &= logits_.ensure((size_t)lrows_cap_ * Vp_ * sizeof(float));
-    ok &= out_dev_.ensure((size_t)lrows_cap_ * (sizeof(SampleOut) + 8 * sizeof(TopkOut)));
-    ok &= out_host_.ensure((size_t)lrows_cap_ * (sizeof(SampleOut) + 8 * sizeof(TopkOut)));
+    ok &= out_dev_.ensure((size_t)lrows_cap_ * (sizeof(SampleOut) + 8 * sizeof(TopkOut) + sizeof(int) + sizeof(float)));       // selections, candidates, draws
+    ok &= out_host_.ensure((size_t)lrows_cap_ * (sizeof(SampleOut) + 8 * sizeof(TopkOut) + sizeof(int) + sizeof(float)));
     ok &= sample_ws_.ensure(sample_workspace_bytes(lrows_cap_));
     logits_host_.assign(V_, 0.0f);
     ok &= ensure_rows(std::max(128, max_seqs));
@@ -162,7 +162,7 @@ bool Engine::ensure_rows(int rows) {
     const size_t R = round_up(rows, 256);
     bool ok = dx_.ensure(R * d_ * sizeof(float)) && dxn_.ensure(R * d_ * sizeof(f16)) && dq_.ensure(R * d_ * sizeof(f16)) &&
               datt_.ensure(R * d_ * sizeof(f16)) && dhid_.ensure(R * 4 * d_ * sizeof(f16));
-    const size_t meta = R * sizeof(DecRow) + (size_t)lrows_cap_ * (sizeof(SampleRow) + sizeof(int) * (kMaxPagesPerSeq + 1)) + 2 * R * sizeof(int2) + 4096;
+    const size_t meta = R * sizeof(DecRow) + (size_t)lrows_cap_ * (sizeof(SampleRow) + sizeof(int) * (kMaxPagesPerSeq + 1 + 5 + 2)) + 2 * R * sizeof(int2) + 4096;
     ok = ok && meta_dev_.ensure(meta) && meta_host_.ensure(meta);
     // split-K partial sums: the largest ws[splits][rows][N] over the four weight shapes of a decoder layer (at d < 853 the
     // QKV and at d < 640 the fc1 projection split too, and their N is 3d and 4d)
@@ -428,7 +428,8 @@ bool Engine::append_kv_slot(Decoder &d, int pos, std::vector<int2> &copies, int 
 
 // ------------------------------------------------------------------------------------------ decoder pass
 bool Engine::decoder_pass(std::vector<DecRow> &rows, const std::vector<SampleRow> &srows, const std::vector<const Decoder *> &seqs,
-                          const std::vector<int2> &page_copies, int T, bool want_raw_logits_host, float *logits_all_out, const LogitsFilter *filter) {
+                          const std::vector<int2> &page_copies, int T, bool want_raw_logits_host, float *logits_all_out, const LogitsFilter *filter,
+                          std::vector<PassDraw> *draws) {
     const int R = (int)rows.size(), L = (int)srows.size(), S = (int)seqs.size(), C = (int)page_copies.size(), d = d_;
     if (R <= 0) return true;
     const double t_pass0 = now_ms();
@@ -449,8 +450,24 @@ bool Engine::decoder_pass(std::vector<DecRow> &rows, const std::vector<SampleRow
         r = e;
     }
     const int NG = (int)xgroups_.size();
+    // draws of the pass, and for passes that feed several tokens of a sequence the first row and the length of each sequence (the rows
+    // of a sequence are consecutive, in the order of seqs and of their positions; checked here, the chunked attention relies on it)
+    const int D = draws ? (int)draws->size() : 0;
+    if (D > lrows_cap_) return false;
+    int max_new = 1;
+    bool chunked = prompt_attention && R > S;
+    seq_start_.assign(S + 1, 0);
+    for (int r = 0; r < R && chunked; r++) {
+        const bool first = r == 0 || rows[r].seq != rows[r - 1].seq;
+        if (first ? rows[r].seq != (r == 0 ? 0 : rows[r - 1].seq + 1) : rows[r].pos != rows[r - 1].pos + 1) chunked = false;
+        else { if (first) seq_start_[rows[r].seq] = r; max_new = std::max(max_new, r - seq_start_[rows[r].seq] + 1); }
+    }
+    chunked = chunked && rows[R - 1].seq == S - 1;
+    seq_start_[S] = R;
+    const int NQ = chunked ? 2 * S + 1 : 0;
     size_t o_rows = 0, o_srow = o_rows + sizeof(DecRow) * R, o_bt = o_srow + sizeof(SampleRow) * L, o_gather = o_bt + sizeof(int) * kMaxPagesPerSeq * S,
-           o_copy = round_up_sz(o_gather + sizeof(int) * L, 8), o_grp = o_copy + sizeof(int2) * C, total = o_grp + sizeof(int2) * NG;
+           o_copy = round_up_sz(o_gather + sizeof(int) * L, 8), o_grp = o_copy + sizeof(int2) * C, o_draw = o_grp + sizeof(int2) * NG,
+           o_chunk = o_draw + 5 * sizeof(int) * D, total = o_chunk + sizeof(int) * NQ;
     if (total > meta_host_.cap) return false;
     memcpy(hb + o_rows, rows.data(), sizeof(DecRow) * R);
     if (L) memcpy(hb + o_srow, srows.data(), sizeof(SampleRow) * L);
@@ -460,10 +477,19 @@ bool Engine::decoder_pass(std::vector<DecRow> &rows, const std::vector<SampleRow
     for (int r = 0; r < R; r++) if (rows[r].logit_row >= 0) gather[rows[r].logit_row] = r;
     if (C) memcpy(hb + o_copy, page_copies.data(), sizeof(int2) * C);
     if (max_group > 1) memcpy(hb + o_grp, xgroups_.data(), sizeof(int2) * NG);
+    for (int i = 0; i < D; i++) {              // logit rows, uniform numbers, top-k, top-p, min-p of the draws
+        int *p = (int *)(hb + o_draw);
+        p[i] = (*draws)[i].logit_row; ((float *)p)[D + i] = (*draws)[i].u; p[2 * D + i] = draw_top_k; ((float *)p)[3 * D + i] = draw_top_p; ((float *)p)[4 * D + i] = draw_min_p;
+    }
+    if (chunked) {
+        int *p = (int *)(hb + o_chunk);
+        memcpy(p, seq_start_.data(), sizeof(int) * (S + 1));
+        for (int s = 0; s < S; s++) p[S + 1 + s] = rows[seq_start_[s + 1] - 1].pos + 1;
+    }
     bool any_probs = false;
-    for (const SampleRow &s : srows) any_probs |= s.want_probs != 0;
+    for (const SampleRow &s : srows) any_probs |= s.want_probs == 1;
     if (L > 0 && any_probs && (!probs_.ensure((size_t)lrows_cap_ * V_ * sizeof(float), false) || !probs_host_.ensure((size_t)lrows_cap_ * V_ * sizeof(float)))) return false;
-    bool any_extra = any_probs;
+    bool any_extra = any_probs || D > 0;
     for (const SampleRow &s : srows) any_extra |= s.topk > 0;
     // Everything the pass puts on its stream, from the metadata upload to the download of the selections. What varies from one
     // pass to the next of the same shape -- tokens, positions, page tables, sampling state -- travels in the metadata buffer, so
@@ -500,6 +526,16 @@ bool Engine::decoder_pass(std::vector<DecRow> &rows, const std::vector<SampleRow
                 PROF(WMI_K_DEC_OTHER, ln_bytes, splitk_residual_ln(x, ws, splits, bias, lw, lb, xn, Rn, d, nullptr, Rn, st));
                 return true;
             };
+            auto self_attention = [&](const f16 *kl, const f16 *vl) -> bool {
+                if (!chunked) return dec_self_attention(q, kl, vl, d_bt, rw, Rn, d, H_, att, st);
+                // prompts: the rows of a sequence share every key they load. (Limits of the text context, not this pass's: a
+                // replayed pass of other lengths is then cut up alike. Neither kernel splits so few keys: no workspace.)
+                const int *starts = (const int *)(db + o_chunk);
+                PagedAttn pa{kl, vl, q, att, d_bt, starts, starts + S + 1, (long)H_ * kPageTokens * 64, 64, kPageTokens * 64, d, 64, d, 64, kMaxPagesPerSeq,
+                             1.0f, WMI_F16, 64, H_, 1, 4, n_pages_, kMaxPagesPerSeq, S, Rn, 0, max_new > 16 ? kMaxTextCtx : 16, kMaxTextCtx};
+                static_assert(kPageTokens == 16, "lp");
+                return paged_attention(pa, nullptr, st);
+            };
             auto cross = [&](int l) -> bool {
                 if (mq && max_grp > 1)      // the group lists hold pass-wide row numbers: buffers from row 0
                     PROF(WMI_K_DEC_CROSS_ATTN, (double)NGn * 2.0 * T * d * 2, dec_cross_attention_mq(dq_.as<f16>(), ckv_.as<f16>(), ckvt_.as<f16>(), d_rows, d_grp + g0, NGn, d, H_, T, Tp_full_, Ld_, l, datt_.as<f16>(), st));
@@ -517,7 +553,7 @@ bool Engine::decoder_pass(std::vector<DecRow> &rows, const std::vector<SampleRow
                 if (few_rows) {
                     auto qw = [&](const QuantW &qq) -> const QuantW * { return quant_decode && qq.ttype ? &qq : nullptr; };
                     PROF(WMI_K_DEC_GEMM, 3 * w1, gemm_rows_ln_dec_qkv(x, D.ln1_w, D.ln1_b, D.wqkv, Rn, d, H_, q, kl, vl, D.bqkv, rw, st, qw(D.q_wqkv)));
-                    PROF(WMI_K_DEC_OTHER, 0, dec_self_attention(q, kl, vl, d_bt, rw, Rn, d, H_, att, st));
+                    PROF(WMI_K_DEC_OTHER, 0, self_attention(kl, vl));
                     PROF(WMI_K_DEC_GEMM, w1, gemm_rows_residual(att, d, D.wo, Rn, d, d, x, d, D.bo, st, qw(D.q_wo)));
                     PROF(WMI_K_DEC_GEMM, w1, gemm_rows_ln_f16(x, D.lnx_w, D.lnx_b, D.xq, Rn, d, d, q, d, D.bxq, 0, 0.125f, st, qw(D.q_xq)));
                     if (!cross(l)) return false;
@@ -533,7 +569,7 @@ bool Engine::decoder_pass(std::vector<DecRow> &rows, const std::vector<SampleRow
                 } else {
                     PROF(WMI_K_DEC_GEMM, 3 * w1, gemm_dec_qkv(xn, D.wqkv, Rn, d, H_, q, kl, vl, D.bqkv, rw, st));
                 }
-                PROF(WMI_K_DEC_OTHER, 0, dec_self_attention(q, kl, vl, d_bt, rw, Rn, d, H_, att, st));
+                PROF(WMI_K_DEC_OTHER, 0, self_attention(kl, vl));
                 if (fused_ln) { if (!residual_ln(att, d, D.wo, D.bo, s_dd, D.lnx_w, D.lnx_b)) return false; }
                 else {
                     PROF(WMI_K_DEC_GEMM, w1, gemm_residual(att, d, D.wo, d, Rn, d, d, x, d, D.bo, st, true));
@@ -573,7 +609,7 @@ bool Engine::decoder_pass(std::vector<DecRow> &rows, const std::vector<SampleRow
         // pass would. The pass's stream forks after the metadata upload and joins before the logits.
         const bool prof_dec = profiling && (profile_mask & ((1u << WMI_K_DEC_GEMM) | (1u << WMI_K_DEC_OTHER) | (1u << WMI_K_DEC_CROSS_ATTN)));
         int cut_row = 0, cut_grp = 0;
-        if (dec_lanes_ > 1 && !prof_dec && R >= 2 * kDecLaneMinRows && lane_stream_ && lane_ws_.p) {
+        if (dec_lanes_ > 1 && !prof_dec && !chunked && R >= 2 * kDecLaneMinRows && lane_stream_ && lane_ws_.p) {
             // cut at the cross-attention group boundary nearest to the middle (rows of one utterance stay in one lane)
             int best = -1;
             for (int gi = 1; gi < NG; gi++) {
@@ -622,6 +658,14 @@ bool Engine::decoder_pass(std::vector<DecRow> &rows, const std::vector<SampleRow
             PROF(WMI_K_DEC_OTHER, 8.0 * L * V_, sample_rows(logits_.as<float>(), Vp_, L, d_srow, model->vocab_ids(), model->nst_bitmap, d_out, d_topk, 8,
                                                            any_probs ? probs_.as<float>() : nullptr, any_extra, sample_ws_.p, stream_));
             WMI_HIP_OK(hipMemcpyAsync(out_host_.p, out_dev_.p, sizeof(SampleOut) * lrows_cap_ + sizeof(TopkOut) * 8 * (size_t)L, hipMemcpyDeviceToHost, stream_));
+            if (D > 0) {
+                const int *m = (const int *)(db + o_draw);
+                const size_t at = (sizeof(SampleOut) + sizeof(TopkOut) * 8) * (size_t)lrows_cap_;
+                int *tok = (int *)(out_dev_.as<char>() + at);
+                const DrawArgs da{logits_.p, nullptr, (const float *)m + 3 * D, (const float *)m + 4 * D, (const float *)m + D, m + 2 * D, m, tok, (float *)tok + D, (long)Vp_, D, V_, WMI_F32};
+                PROF(WMI_K_DEC_OTHER, 4.0 * D * V_, draw_tokens(da, stream_));
+                WMI_HIP_OK(hipMemcpyAsync(out_host_.as<char>() + at, tok, (sizeof(int) + sizeof(float)) * (size_t)D, hipMemcpyDeviceToHost, stream_));
+            }
             if (any_probs) WMI_HIP_OK(hipMemcpyAsync(probs_host_.p, probs_.p, sizeof(float) * (size_t)L * V_, hipMemcpyDeviceToHost, stream_));
         }
         return true;
@@ -637,7 +681,7 @@ bool Engine::decoder_pass(std::vector<DecRow> &rows, const std::vector<SampleRow
         for (const void *q : {dx_.p, dxn_.p, dq_.p, datt_.p, dhid_.p, dxl_.p, logits_.p, meta_dev_.p, (void *)meta_host_.p, out_dev_.p, (void *)out_host_.p, ckv_.p, ckvt_.p,
                               kpool_.p, vpool_.p, splitk_ws_.p, sample_ws_.p})
             ptrs = ptrs * 1000003u ^ (uintptr_t)q;
-        const PassKey key{{R, L, S, C, NG, max_group, T, (int)any_extra | (mq ? 2 : 0) | (quant_decode ? 4 : 0), (int)(ptrs & 0x7fffffff), (int)((ptrs >> 31) & 0x7fffffff)}};
+        const PassKey key{{R, L, S, C, NG, max_group, T, (int)any_extra | (mq ? 2 : 0) | (quant_decode ? 4 : 0) | (chunked ? (max_new > 16 ? 8 : 16) : 0) | (D << 5), (int)(ptrs & 0x7fffffff), (int)((ptrs >> 31) & 0x7fffffff)}};
         if (graphs_.size() > 64) clear_graphs();
         PassGraph &g = graphs_[key];
         if (g.exec) {
@@ -663,6 +707,10 @@ bool Engine::decoder_pass(std::vector<DecRow> &rows, const std::vector<SampleRow
     if (!launched && !enqueue()) return false;
     const double t_launched = now_ms();
     WMI_HIP_OK(hipStreamSynchronize(stream_));
+    if (D > 0) {
+        const int *tok = (const int *)(out_host_.as<char>() + (sizeof(SampleOut) + sizeof(TopkOut) * 8) * (size_t)lrows_cap_);
+        for (int i = 0; i < D; i++) { (*draws)[i].id = tok[i]; (*draws)[i].plog = ((const float *)tok)[D + i]; }
+    }
     t_dec_launch_ms += t_launched - t_pass0; t_dec_wait_ms += now_ms() - t_launched; n_passes++;
     n_decode += R;
     return true;
@@ -783,9 +831,10 @@ struct Engine::Run {
         uint64_t h = 0x6d656d6full;
         const int iv[] = {P.strategy, P.n_max_text_ctx, P.offset_ms, P.duration_ms, P.translate, P.no_context, P.no_timestamps, P.single_segment, P.print_special,
                           P.max_tokens, P.audio_ctx, P.tdrz_enable, P.suppress_blank, P.suppress_nst, P.greedy.best_of, P.beam_search.beam_size,
-                          E.force_tokens, (int)E.beam_sampled, n_decoders, P.token_timestamps, P.max_len, P.split_on_word};
+                          E.device_draws ? 1 + E.draw_top_k : 0, (int)E.prompt_attention, E.force_tokens, (int)E.beam_sampled, n_decoders, P.token_timestamps, P.max_len, P.split_on_word};
         h = hash_bytes(iv, sizeof iv, h);
-        const float fv[] = {P.temperature, P.max_initial_ts, P.length_penalty, P.temperature_inc, P.entropy_thold, P.logprob_thold, P.no_speech_thold, P.beam_search.patience};
+        const float fv[] = {P.temperature, P.max_initial_ts, P.length_penalty, P.temperature_inc, P.entropy_thold, P.logprob_thold, P.no_speech_thold, P.beam_search.patience,
+                            E.device_draws ? E.draw_top_p : 1.0f, E.device_draws ? E.draw_min_p : 0.0f};
         h = hash_bytes(fv, sizeof fv, h);
         if (!initial_prompt_tokens.empty()) h = hash_bytes(initial_prompt_tokens.data(), initial_prompt_tokens.size() * sizeof(int), h);
         return h;
@@ -954,7 +1003,7 @@ struct Engine::Run {
         s.n_sampled = n; s.force_n = E.force_tokens;
         const bool beam = P.strategy == WHISPER_SAMPLING_BEAM_SEARCH;
         s.topk = (beam && !E.beam_sampled) ? std::min(8, P.beam_search.beam_size) : 0;
-        s.want_probs = ((!beam && u.t_cur > 0.0f) || (beam && E.beam_sampled)) ? 1 : 0;
+        s.want_probs = !beam && u.t_cur > 0.0f ? (E.device_draws ? 2 : 1) : beam && E.beam_sampled ? 1 : 0;
         return s;
     }
 
@@ -969,6 +1018,7 @@ struct Engine::Run {
             if (P.strategy == WHISPER_SAMPLING_GREEDY) {
                 whisper_token_data t;
                 if (u.t_cur < 1e-6f) t = make_token(d.so.id, d.so.tid, d.so.p, d.so.plog, d.so.pt, d.so.ptsum, beg);
+                else if (E.device_draws) t = make_token(d.draw_id, d.so.tid, expf(d.draw_plog), d.draw_plog, d.so.pt, d.so.ptsum, beg);
                 else { const int id = sample_discrete(d.probs.data(), E.V_, d.rng); const float p = d.probs[id]; t = make_token(id, d.so.tid, p, logf(p), d.so.pt, d.so.ptsum, beg); }
                 d.seq.tokens.push_back(t); d.seq.sum_logprobs_all += t.plog;
             } else {
@@ -1170,7 +1220,8 @@ int Engine::Run::run_group(const float *const *pcm, const int *n, int g0, int G,
     E.t_mel_ms += now_ms() - t0;
 
     std::vector<DecRow> rows; std::vector<SampleRow> srows; std::vector<const Decoder *> seqs; std::vector<int2> copies;
-    std::vector<PassRowRef> lref;
+    std::vector<PassRowRef> lref, draw_ref;
+    std::vector<PassDraw> draws;
     std::vector<char> in_pass, gated;
     E.enc_events_used_ = 0;
     int rc = 0;
@@ -1319,7 +1370,16 @@ int Engine::Run::run_group(const float *const *pcm, const int *n, int g0, int G,
                 const std::vector<whisper_token_data> &tk = fu.dec[lref[lr].dec].seq.tokens;
                 P.logits_filter_callback(ctx, st, tk.data(), fu.phase == Phase::Prompt ? 0 : (int)tk.size(), logits, P.logits_filter_callback_user_data);
             };
-        if (!E.decoder_pass(rows, srows, seqs, copies, T, false, nullptr, P.logits_filter_callback ? &filter : nullptr)) { rc = -7; break; }
+        // draws on the device: every decoder that takes a token from a row of this pass, with a number of its own generator (after a
+        // prompt all of an utterance's decoders draw from its one row)
+        draws.clear(); draw_ref.clear();
+        for (size_t lr = 0; lr < lref.size(); lr++) {
+            if (srows[lr].want_probs != 2) continue;
+            Utt &u = utts[lref[lr].utt];
+            const int j0 = u.phase == Phase::Prompt ? 0 : lref[lr].dec, j1 = u.phase == Phase::Prompt ? u.n_cur : j0 + 1;
+            for (int j = j0; j < j1; j++) { draws.push_back(PassDraw{(int)lr, (float)(u.dec[j].rng() >> 8) * 0x1p-24f, 0, 0.0f}); draw_ref.push_back({lref[lr].utt, j}); }
+        }
+        if (!E.decoder_pass(rows, srows, seqs, copies, T, false, nullptr, P.logits_filter_callback ? &filter : nullptr, &draws)) { rc = -7; break; }
         E.t_decode_ms += now_ms() - t0;
         const SampleOut *so = E.out_host_.as<SampleOut>();
         const TopkOut *tk = (const TopkOut *)(E.out_host_.as<char>() + sizeof(SampleOut) * E.lrows_cap_);
@@ -1329,8 +1389,9 @@ int Engine::Run::run_group(const float *const *pcm, const int *n, int g0, int G,
             Decoder &d = u.dec[lref[lr].dec];
             d.so = so[lr];
             for (int c = 0; c < 8; c++) d.topk[c] = tk[lr * 8 + c];
-            if (srows[lr].want_probs) d.probs.assign(E.probs_host_.as<float>() + lr * (size_t)E.V_, E.probs_host_.as<float>() + (lr + 1) * (size_t)E.V_);
+            if (srows[lr].want_probs == 1) d.probs.assign(E.probs_host_.as<float>() + lr * (size_t)E.V_, E.probs_host_.as<float>() + (lr + 1) * (size_t)E.V_);
         }
+        for (size_t i = 0; i < draws.size(); i++) { Decoder &d = utts[draw_ref[i].utt].dec[draw_ref[i].dec]; d.draw_id = draws[i].id >= 0 ? draws[i].id : d.so.id; d.draw_plog = draws[i].plog; }   // (-1: the rules left nothing)
         // ---- advance the state machines of the utterances that were in the pass
         for (int i = 0; i < G; i++) {
             Utt &u = utts[i];

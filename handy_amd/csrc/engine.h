@@ -56,6 +56,8 @@ struct Decoder {
     SampleOut so{};              // selection computed from the latest logits of this sequence
     TopkOut topk[8];
     std::vector<float> probs;    // full probability row when the host has to draw from it
+    int draw_id = 0;             // token drawn on the device (device_draws) and its log-probability
+    float draw_plog = 0;
 };
 
 enum class Phase { LangEncode, LangDecode, Encode, Prompt, Step, Done };
@@ -95,6 +97,8 @@ struct WindowMemo {
     std::vector<std::mt19937> rng;
 };
 
+// one draw of a decoder pass: which logit row it looks at and its uniform number; the token and log-probability come back
+struct PassDraw { int logit_row; float u; int id; float plog; };
 struct PassRowRef { int utt, dec; };   // which (utterance, decoder) a logit row belongs to
 
 class Engine {
@@ -130,6 +134,10 @@ public:
     int encoder_lanes = 1;               // 2: alternate encoder chunks between two streams/workspaces
     bool set_encoder_lanes(int n);
     bool beam_sampled = false;
+    bool device_draws = false;           // draws at a temperature happen on the device (draw_tokens), with these filters
+    int draw_top_k = 0;
+    float draw_top_p = 1.0f, draw_min_p = 0.0f;
+    bool prompt_attention = false;       // passes that feed several tokens of a sequence use the chunked attention (paged_attention)
     int exp_n_audio_ctx = 0;
 
     // profiling
@@ -199,6 +207,7 @@ private:
     std::vector<float> filter_rows_;  // logit rows on the host while the caller's logits_filter_callback looks at them
     Decoder ll_dec_;                 // sequence used by whisper_decode()
     std::vector<int2> xgroups_;      // cross-attention row groups of the pass being built
+    std::vector<int> seq_start_;     // first row of every sequence of the pass being built
 
     // decoder passes replayed as HIP graphs, by pass shape (decoder_pass)
     struct PassKey { std::array<int, 10> v; bool operator<(const PassKey &o) const { return v < o.v; } };
@@ -223,7 +232,8 @@ private:
     // filter (optional): called per logit row with that row's logits in host memory, between the two halves of the rules
     using LogitsFilter = std::function<void(int logit_row, float *logits)>;
     bool decoder_pass(std::vector<DecRow> &rows, const std::vector<SampleRow> &srows, const std::vector<const Decoder *> &seqs,
-                      const std::vector<int2> &page_copies, int T, bool want_raw_logits_host, float *logits_all_out, const LogitsFilter *filter = nullptr);
+                      const std::vector<int2> &page_copies, int T, bool want_raw_logits_host, float *logits_all_out, const LogitsFilter *filter = nullptr,
+                      std::vector<PassDraw> *draws = nullptr);
     // KV pages
     int page_alloc();
     void page_release(std::vector<int> &pages);

@@ -474,7 +474,7 @@ __global__ __launch_bounds__(64) void sample_final_kernel(const SamplePartial *_
 
 struct TopkCand { float v; int i; };
 
-__global__ __launch_bounds__(256) void sample_extra_kernel(const float *__restrict__ logits, long ld, const SampleRow *__restrict__ srow, VocabIds vi,
+__global__ __launch_bounds__(256) void sample_extra_kernel(float *__restrict__ logits, long ld, const SampleRow *__restrict__ srow, VocabIds vi,
                                                            const SampleOut *__restrict__ out, float *__restrict__ probs, TopkCand *__restrict__ cand) {
     __shared__ ArgMax sh_a[4];
     const int s = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, V = vi.n_vocab;
@@ -482,15 +482,15 @@ __global__ __launch_bounds__(256) void sample_extra_kernel(const float *__restri
     if (!sr.want_probs && sr.topk <= 0) return;
     const SampleOut o = out[r];
     const bool ts_wins = o.pad != 0;
-    const float *lg = logits + (long)r * ld;
+    float *lg = logits + (long)r * ld;
     float val[kSamplePer];
 #pragma unroll
     for (int k = 0; k < kSamplePer; k++) {
         const int i = s * kSampleChunk + k * 256 + tid;
         float v = -INFINITY;
-        if (i < V) { v = lg[i]; if (ts_wins && i < vi.beg) v = -INFINITY; }
+        if (i < V) { v = lg[i]; if (ts_wins && i < vi.beg) { v = -INFINITY; if (sr.want_probs == 2) lg[i] = v; } }
         val[k] = v;
-        if (probs && sr.want_probs && i < V) probs[(long)r * V + i] = v == -INFINITY ? 0.0f : __expf(v - o.lse);
+        if (probs && sr.want_probs == 1 && i < V) probs[(long)r * V + i] = v == -INFINITY ? 0.0f : __expf(v - o.lse);
     }
     if (cand && sr.topk > 0) {
         for (int t = 0; t < sr.topk && t < 8; t++) {

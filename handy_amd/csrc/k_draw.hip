@@ -91,7 +91,7 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
     constexpr int W = TH / 64, U = 4;
     __shared__ DrawShared<TH> sh;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), V = a.n_vocab;
-    const T *src = (const T *)a.logits + row * a.row_stride;
+    const T *src = (const T *)a.logits + (a.row_of ? a.row_of[row] : row) * a.row_stride;
     const float t_in = a.temperature ? a.temperature[row] : 1.0f, p_in = a.top_p ? a.top_p[row] : 1.0f, m_in = a.min_p ? a.min_p[row] : 0.0f, u_in = a.uniform[row];
     const int k_in = a.top_k ? a.top_k[row] : 0;
     const int run = ((V + W - 1) / W + 255) & ~255;          // entries of a wave
@@ -593,7 +593,7 @@ WHISPER_API int wmi_sample_tokens(const void *logits, int dtype, long long row_s
     if (!call.ok()) return -4;
     if (!call.own(logits, (const void *)uniform, (const void *)token) || (temperature && !call.owns(temperature)) || (top_k && !call.owns(top_k)) ||
         (top_p && !call.owns(top_p)) || (min_p && !call.owns(min_p)) || (logprob && !call.owns(logprob))) return -1;
-    const DrawArgs a{logits, temperature, top_p, min_p, uniform, top_k, token, logprob, (long)row_stride, n_rows, n_vocab, dtype};
+    const DrawArgs a{logits, temperature, top_p, min_p, uniform, top_k, nullptr, token, logprob, (long)row_stride, n_rows, n_vocab, dtype};
     return draw_tokens(a, st) ? 0 : -4;
 }
 

@@ -112,6 +112,7 @@ bool dec_cross_attention(const f16 *q, const f16 *ckv, const DecRow *rows, const
                          int n_layer, int layer, f16 *att, hipStream_t st);
 // logits rules + log-softmax + argmax / top-k / probabilities for every logit row
 // (the masked logits are written back in place; nst_bitmap has one bit per token id)
+// want_probs 2: text tokens that the timestamp rule outweighs are masked in place as well, so that the row is what to draw from
 // any_extra: some row has topk > 0 or want_probs; workspace: sample_workspace_bytes(max rows) of device memory
 size_t sample_workspace_bytes(int max_rows);
 bool sample_rows(float *logits, long ld, int R, const SampleRow *srow, const VocabIds &vi, const unsigned *nst_bitmap,
@@ -147,6 +148,7 @@ struct DrawArgs {
     const float *temperature, *top_p, *min_p;                    // null: 1, off, off
     const float *uniform;
     const int *top_k;                                             // null: off
+    const int *row_of;                                            // row of the logits each draw looks at; null: draw i, row i
     int *token;
     float *logprob;                                               // null: not wanted
     long row_stride;

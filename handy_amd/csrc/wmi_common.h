@@ -103,7 +103,7 @@ struct SampleRow {
     int32_t n_sampled;      // tokens sampled so far in this sequence
     int32_t force_n;        // benchmark control: >0 => no EOT before, only EOT at, this many tokens
     int32_t topk;           // 0: argmax only; k>0: also write the k most probable tokens
-    int32_t want_probs;     // 1: write the full probability row (host-side sampling at T>0)
+    int32_t want_probs;     // 1: write the full probability row (host-side sampling at T>0); 2: leave the row ready for draw_tokens
 };
 
 struct SampleOut {          // one per logit row

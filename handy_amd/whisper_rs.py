@@ -149,7 +149,7 @@ wmi_batch_segment_text wmi_batch_n_tokens wmi_batch_token_data wmi_batch_lang_id
 wmi_set_force_tokens wmi_set_beam_candidates_sampled wmi_mel_batch_device wmi_mel_batch_device_normalized wmi_pcm_to_mel_device_noalloc wmi_get_mel wmi_get_encoder_output wmi_get_cross_kv
 wmi_decode_logits_all wmi_debug_gemm wmi_debug_gemm_gelu wmi_debug_expand_blocks wmi_debug_quant_rows wmi_debug_enc_attention wmi_set_window_cache wmi_get_window_cache_stats wmi_set_pipeline_groups wmi_set_encoder_lanes wmi_set_profiling wmi_set_profiling_classes wmi_get_kernel_stats wmi_reset_kernel_stats wmi_get_host_timings wmi_set_quant_decode wmi_set_quant_resident wmi_set_decoder_lanes wmi_set_pass_graphs wmi_version
 wmi_ingest_n_frames wmi_ingest_resample wmi_ingest_gate_plan wmi_ingest_gather
-wmi_paged_plan wmi_paged_write wmi_paged_attention_workspace wmi_paged_attention wmi_sample_tokens
+wmi_set_device_draws wmi_set_prompt_attention wmi_paged_plan wmi_paged_write wmi_paged_attention_workspace wmi_paged_attention wmi_sample_tokens
 wmi_ctx_for_device wmi_node_init wmi_node_free wmi_node_n_devices wmi_node_state wmi_node_context wmi_node_run wmi_node_last_gather
 wmi_node_last_batches wmi_node_run_custom
 wmi_dev_alloc wmi_dev_free wmi_dev_upload wmi_dev_download wmi_dev_memset wmi_dev_sync wmi_dev_free_bytes wmi_dev_stream_create
@@ -227,6 +227,8 @@ def load_library(path: Optional[str] = None):
     L.wmi_batch_n_fallbacks.restype = ci; L.wmi_batch_n_fallbacks.argtypes = [vp, ci]
     L.wmi_batch_rc.restype = ci; L.wmi_batch_rc.argtypes = [vp, ci]
     L.wmi_set_force_tokens.argtypes = [vp, ci]; L.wmi_set_beam_candidates_sampled.argtypes = [vp, ci]
+    L.wmi_set_device_draws.restype = ci; L.wmi_set_device_draws.argtypes = [vp, ci, ci, C.c_float, C.c_float]
+    L.wmi_set_prompt_attention.restype = ci; L.wmi_set_prompt_attention.argtypes = [vp, ci]
     L.wmi_mel_batch_device.restype = ci; L.wmi_mel_batch_device.argtypes = [vp, vp, vp, C.POINTER(C.c_longlong), C.POINTER(ci), ci]
     L.wmi_mel_batch_device_normalized.restype = ci; L.wmi_mel_batch_device_normalized.argtypes = [vp, vp, vp, C.POINTER(C.c_longlong), C.POINTER(ci), ci, vp, ci]
     L.wmi_pcm_to_mel_device_noalloc.restype = ci; L.wmi_pcm_to_mel_device_noalloc.argtypes = [vp, vp, ci, vp, ci, vp]
@@ -587,6 +589,12 @@ class WhisperState:
     # -- knobs / stats
     def set_force_tokens(self, n: int): self.L.wmi_set_force_tokens(self.h, n)
     def set_beam_candidates_sampled(self, v: bool): self.L.wmi_set_beam_candidates_sampled(self.h, int(v))
+    def set_device_draws(self, on: bool, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0):
+        """Draws at a temperature on the GPU, with top-k, top-p and min-p (see wmi_set_device_draws)."""
+        if self.L.wmi_set_device_draws(self.h, int(on), top_k, top_p, min_p) != 0: raise WhisperError("GenericError", -1)
+    def set_prompt_attention(self, on: bool):
+        """Chunked self-attention for passes that feed several tokens of a sequence (see wmi_set_prompt_attention)."""
+        if self.L.wmi_set_prompt_attention(self.h, int(on)) != 0: raise WhisperError("GenericError", -1)
     def set_profiling(self, on: bool): self.L.wmi_set_profiling(self.h, int(on))
     def set_pipeline_groups(self, n: int): self.L.wmi_set_pipeline_groups(self.h, int(n))
 

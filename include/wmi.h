@@ -66,6 +66,17 @@ WHISPER_API int wmi_set_encoder_lanes(struct whisper_state *state, int n);
 /* Beam-search candidate rule: 0 = deterministic k most probable tokens per beam (default),
  * 1 = k draws from the token distribution with a per-decoder mt19937 (what upstream does). */
 WHISPER_API void wmi_set_beam_candidates_sampled(struct whisper_state *state, int sampled);
+/* on != 0: the greedy strategy's draws at a temperature above 0 (the fallback's best_of sequences) are made on the GPU by
+ * wmi_sample_tokens' kernel instead of on the host: no probability rows cross the bus (207 KB a sequence and token for a
+ * 51 866-entry vocabulary), and top_k (0: off), top_p (1: off) and min_p (0: off) narrow them down. Every sequence still draws from
+ * its own mt19937 (one number a token, not two), so the transcripts at a temperature are others than with the host's draws, and the
+ * same on every run; a token's probability is the one among what the rules leave. Off by default. Returns 0, -1 for bad arguments. */
+WHISPER_API int wmi_set_device_draws(struct whisper_state *state, int on, int top_k, float top_p, float min_p);
+/* on != 0: decoder passes that feed several tokens of a sequence (prompts with text context, whisper_decode of more than one
+ * token) use wmi_paged_attention's kernels for the self-attention of all their rows: the rows of a sequence share the keys they
+ * load. The probabilities are then rounded to fp16 for the product with V, which the single-row kernel does not do: logits agree
+ * to fp16 accuracy, not to the bit, and a row's may depend on whether a prompt shares its pass. Off by default. Returns 0 or -1. */
+WHISPER_API int wmi_set_prompt_attention(struct whisper_state *state, int on);
 
 /* Log-mel only, for n_utts utterances already in DEVICE memory (pcm_dev + offsets[i], n_samples[i] floats):
  * runs the frontend kernels and leaves the raw log-mel on the device. Used by the mel roofline probe. */

@@ -280,6 +280,8 @@ extern "C" {
     pub fn wmi_set_encoder_lanes(state: *mut whisper_state, n: c_int) -> c_int;
     pub fn wmi_set_decoder_lanes(state: *mut whisper_state, n: c_int) -> c_int;
     pub fn wmi_set_pass_graphs(state: *mut whisper_state, on: c_int);
+    pub fn wmi_set_device_draws(state: *mut whisper_state, on: c_int, top_k: c_int, top_p: c_float, min_p: c_float) -> c_int;
+    pub fn wmi_set_prompt_attention(state: *mut whisper_state, on: c_int) -> c_int;
     pub fn wmi_set_beam_candidates_sampled(state: *mut whisper_state, sampled: c_int);
     pub fn wmi_set_quant_resident(on: c_int);
     pub fn wmi_set_quant_decode(state: *mut whisper_state, on: c_int) -> c_int;
