@@ -826,6 +826,13 @@ WHISPER_API int wmi_paged_plan(const int *ctx_lens, const int *new_lens, int n_s
     if (n_seq > 0 && (!ctx_lens || !new_lens || !kv_lens)) return -1;
     if ((n_seq > 0 && table_cols > 0 && !block_table) || (n_free > 0 && !free_pages) || (n_rows_cap > 0 && (!slots || !positions))) return -1;
     if (!power_of_two(page_tokens) || page_tokens > 1024 || n_seq > kPlanMaxSeq || (long long)table_cols * page_tokens > 0x7fffffffLL) return -3;
+    // Workgroups read all lengths while others write: what is written overlaps nothing else (the last plan's kv_lens as this one's
+    // ctx_lens in the same buffer would).
+    const struct { const void *p; long long n; } use[] = {{ctx_lens, n_seq}, {new_lens, n_seq}, {free_pages, n_free}, {block_table, n_seq > 0 && table_cols > 0 ? (n_seq - 1) * table_stride + table_cols : 0},
+                                                          {cu_q, n_seq + 1LL}, {kv_lens, n_seq}, {slots, n_rows_cap}, {positions, n_rows_cap}, {counts, 4}};
+    for (int i = 3; i < 9; i++)
+        for (int j = 0; j < i; j++)
+            if (use[i].n > 0 && use[j].n > 0 && (uintptr_t)use[i].p < (uintptr_t)use[j].p + 4 * use[j].n && (uintptr_t)use[j].p < (uintptr_t)use[i].p + 4 * use[i].n) return -1;
     hipStream_t st = (hipStream_t)stream;
     const ServeCall call(st);
     if (!call.ok()) return -4;
@@ -846,6 +853,7 @@ WHISPER_API int wmi_paged_write(const wmi_paged_cache *cache, const void *k_new,
     if (rc) return rc;
     if (n_rows < 0 || (n_rows > 0 && (!k_new || !v_new || !slots)) || k_row_stride < 0 || k_head_stride < 0 || v_row_stride < 0 || v_head_stride < 0) return -1;
     if (n_rows == 0) return 0;
+    if (cache->k == cache->v && (k_new != v_new || k_row_stride != v_row_stride || k_head_stride != v_head_stride)) return -1;      // two values for one place
     hipStream_t st = (hipStream_t)stream;
     const ServeCall call(st);
     if (!call.ok()) return -4;

@@ -178,7 +178,8 @@ class PagePlan:
 
 def plan_pages(ctx_lens, new_lens, free_pages, block_table, page_tokens: int, out: PagePlan, stream: int = 0) -> PagePlan:
     """Admit requests in order, give them fresh pages from the front of free_pages (entered in block_table[n_seq, cols]) and number
-    their rows: see wmi_paged_plan in include/wmi.h. The number of rows planned for is the length of out.slots."""
+    their rows: see wmi_paged_plan in include/wmi.h. The number of rows planned for is the length of out.slots. The plan's arrays and
+    block_table share no memory with each other or the inputs (copy out.kv_lens for the next step's ctx_lens)."""
     n_seq, n_free = out.n_seq, free_pages.shape[0]
     tp, stride, cols = _table(block_table, n_seq)
     if ctx_lens.shape[0] != n_seq or new_lens.shape[0] != n_seq:
@@ -224,8 +225,11 @@ def paged_attention(q, cache: PagedCache, block_table, cu_q, kv_lens, max_new: i
     op, orow, oh = _rows(out, shape, cache.dtype, "out")
     n_seq = kv_lens.shape[0]
     tp, stride, cols = _table(block_table, n_seq)
-    a = _ATTN.pack(qp or 0, op or 0, tp or 0, _flat(cu_q, "int32", n_seq + 1, "cu_q") or 0, _flat(kv_lens, "int32", n_seq, "kv_lens") or 0, qr, qh, orow, oh, stride, cols,
-                   shape[0], n_seq, shape[1], window, max_new, max_kv, dim ** -0.5 if scale is None else scale)
+    try:
+        a = _ATTN.pack(qp or 0, op or 0, tp or 0, _flat(cu_q, "int32", n_seq + 1, "cu_q") or 0, _flat(kv_lens, "int32", n_seq, "kv_lens") or 0, qr, qh, orow, oh, stride, cols,
+                       shape[0], n_seq, shape[1], window, max_new, max_kv, dim ** -0.5 if scale is None else scale)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"paged_attention: {e}") from None
     ws, ws_bytes = None, 0
     if workspace is not None:
         ws_bytes = workspace.shape[0]

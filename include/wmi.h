@@ -287,12 +287,12 @@ typedef struct wmi_paged_cache {
  *   positions[n_rows_cap]  position of each row in its sequence (0 past the last)
  *   counts[4]         {requests admitted (index of the first that was not), rows, fresh pages taken, requests passed over}
  * Entries of block_table that no fresh page goes to are left as they are; the call may be repeated on its own result.
- * n_seq <= 16384. */
+ * n_seq <= 16384. Outputs and block_table overlap neither each other nor an input (-1): the next step's ctx_lens are a copy. */
 WHISPER_API int wmi_paged_plan(const int *ctx_lens, const int *new_lens, int n_seq, const int *free_pages, int n_free, int page_tokens, int *block_table,
                                int table_cols, long long table_stride, int *cu_q, int *kv_lens, int *slots, int *positions, int n_rows_cap, int *counts, void *stream);
 
 /* cache[slots[r]] = (k_new, v_new)[r], rows [n_kv_heads][head_dim] at the given strides in the cache's type; a row whose slot
- * is negative or past the cache is skipped. The slots of one call must be distinct. */
+ * is negative or past the cache is skipped. The slots of one call must be distinct, and the rows read not among those written. */
 WHISPER_API int wmi_paged_write(const wmi_paged_cache *cache, const void *k_new, long long k_row_stride, long long k_head_stride, const void *v_new,
                                 long long v_row_stride, long long v_head_stride, const int *slots, int n_rows, void *stream);
 
@@ -300,10 +300,10 @@ WHISPER_API int wmi_paged_write(const wmi_paged_cache *cache, const void *k_new,
  * kv_lens[i] tokens: row t of n stands at position kv_lens[i] - n + t and sees the keys up to its own position, with window > 0
  * only the last `window` of them. Query heads share key heads in runs of n_q_heads / n_kv_heads (<= 128). Keys on pages that the
  * cache does not have (table entry negative or >= n_pages) are left out; a row that sees no key gives zeros; rows past
- * cu_q[n_seq] are left as they are. head_dim a multiple of 8 up to 128; 16-byte aligned pointers, strides multiples of 8.
+ * cu_q[n_seq] are left as they are. out shares no memory with what is read. head_dim a multiple of 8 up to 128; 16-byte aligned pointers, strides multiples of 8.
  * max_new and max_kv: the longest request's new and total tokens, as far as the caller knows (they steer how the work is split,
  * larger or smaller values change no result beyond rounding; 0: not known). Scores, softmax and sums are 32-bit; the
- * probabilities are rounded to the cache's type for the product with V. */
+ * probabilities are rounded to the cache's type for the product with V. An infinite V may come out as NaN in the rows that see it. */
 typedef struct wmi_paged_attn {
     const void *q;             /* [n_rows][n_q_heads][head_dim], the cache's type */
     void *out;                 /* the same shape and type */

@@ -136,3 +136,34 @@ def test_restatement_on_cases_worked_by_hand():
     k = np.zeros((1, 4, 1, 2)); v = np.arange(8.0).reshape(1, 4, 1, 2)
     out, _, _ = so.attention(np.zeros((2, 1, 2)), k, v, np.array([[0]]), [0, 2], [3], 4, 1.0)
     assert out[:, 0].tolist() == [[1.0, 2.0], [2.0, 3.0]]                             # means of the first two and three values
+
+
+def test_plan_and_write_refuse_shared_memory():
+    """Outputs that overlap an input or each other (workgroups read the lengths while others write), and one place for K and V."""
+    L = wr.load_library()
+    names = ["ctx", "new", "free", "table", "cu", "kv", "slots", "pos", "counts"]
+    def plan(**kw):
+        a = dict(zip(names, (0x10000 * (i + 1) for i in range(9))))
+        a.update(kw)
+        return L.wmi_paged_plan(a["ctx"], a["new"], 3, a["free"], 2, 16, a["table"], 4, 5, a["cu"], a["kv"], a["slots"], a["pos"], 6, a["counts"], None)
+    base = dict(zip(names, (0x10000 * (i + 1) for i in range(9))))
+    size = dict(ctx=3, new=3, free=2, table=14, cu=4, kv=3, slots=6, pos=6, counts=4)
+    for out in names[3:]:
+        for other in names:
+            if other == out:
+                continue
+            for at in (base[other], base[other] + 4 * (size[other] - 1), base[other] - 4 * (size[out] - 1)):      # equal, and by one entry at either end
+                assert plan(**{out: at}) == -1, (out, other)
+    assert L.wmi_paged_write(C.byref(cache_struct(k=P, v=P)), 0x20000, 128, 64, 0x30000, 128, 64, 0x40000, 3, None) == -1
+    assert L.wmi_paged_write(C.byref(cache_struct(k=P, v=P)), 0x20000, 128, 64, 0x20000, 256, 64, 0x40000, 3, None) == -1
+
+
+def test_numbers_out_of_range_are_value_errors():
+    cache = sv.PagedCache(Fake((8, 16, 2, 64), "float16"), Fake((8, 16, 2, 64), "float16"))
+    i32 = lambda *s: Fake(s, "int32")
+    q, out = Fake((5, 4, 64), "float16"), Fake((5, 4, 64), "float16")
+    for kw in (dict(window=2 ** 31), dict(window=-2 ** 40), dict(scale=1e300), dict(window=1.5)):
+        with pytest.raises(ValueError):
+            sv.paged_attention(q, cache, i32(3, 8), i32(4), i32(3), 1, 100, out, **kw)
+    with pytest.raises(ValueError):
+        sv.paged_attention(q, cache, i32(3, 8), i32(4), i32(3), 1, 2 ** 33, out)

@@ -511,3 +511,71 @@ def test_host_memory_is_refused_and_nothing_runs():
     assert np.array_equal(bases[0].numpy(), before)
     assert L.wmi_sample_tokens(x.data_ptr(), 2, 50, 2, 50, u.data_ptr(), None, None, None, None, tok.data_ptr(), None, None) == 0      # and the next call runs
     assert L.wmi_dev_sync() == 0 and (tok.numpy() == 0).all()
+
+
+@pytest.mark.parametrize("head_major", [False, True])
+def test_offsets_past_32_bits_in_a_long_cache(head_major):
+    """A cache of more than 2^32 elements (9.7 GB each of K and V): pages at its end are written and read, nothing at their offsets
+    modulo 2^31 or 2^32."""
+    dtype, page, hkv, dim, n_pages = "float16", 16, 8, 128, 296000
+    per = page * hkv * dim
+    assert n_pages * per > 2 ** 32 + 2 ** 28
+    bases = [sv.DeviceArray((n_pages, page, hkv, dim), dtype) for _ in range(2)]
+    strides = (per, dim, page * dim, 1) if head_major else (per, hkv * dim, dim, 1)
+    cache = sv.PagedCache(*(b.view((n_pages, page, hkv, dim), strides) for b in bases))
+    rng = np.random.default_rng(2)
+    L, lens = wr.load_library(), [150, 31]
+    pages = np.array([n_pages - 1 - 3 * i for i in range(12)], np.int32)
+    table = np.full((2, 10), -1, np.int32)
+    table[0], table[1, :2] = pages[:10], pages[10:]
+    low = sorted({(int(p) * per) % m // per + d for p in pages for m in (2 ** 31, 2 ** 32) for d in (0, 1)})       # what a 32-bit offset would hit
+    zeros = np.zeros(per, np.float16)
+    for b in bases:
+        for p in low + pages.tolist():
+            assert L.wmi_dev_upload(b.data_ptr() + p * per * 2, zeros.ctypes.data, zeros.nbytes) == 0
+    new = [rng.standard_normal((sum(lens), hkv, dim)).astype(np.float16) for _ in range(2)]
+    slots = np.concatenate([[table[i, j // page] * page + j % page for j in range(n)] for i, n in enumerate(lens)]).astype(np.int32)
+    sv.write_kv(cache, dev(new[0]), dev(new[1]), dev(slots))
+    got = np.empty(per, np.float16)
+    for which, b in enumerate(bases):
+        for p in low:
+            assert L.wmi_dev_download(got.ctypes.data, b.data_ptr() + p * per * 2, got.nbytes) == 0 and not got.any(), p
+    hosts = [np.zeros((n_pages - int(pages.min()), page, hkv, dim), np.float16) for _ in range(2)]
+    for h, x in zip(hosts, new):
+        h[(slots // page) - int(pages.min()), slots % page] = x
+    small = np.where(table >= 0, table - pages.min(), -1)
+    for news in ([1, 1], [70, 31]):
+        q = (rng.standard_normal((sum(news), hkv * 2, dim))).astype(np.float16)
+        cu = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
+        out = run_attn(cache, table, q, cu, np.array(lens, np.int32), dtype, max(news), max(lens))
+        check_attn(out, dtype, q, hosts, small, cu, lens, page, dim ** -0.5, what=str(news))
+    for b in bases:
+        b.free()
+
+
+def test_calls_on_two_streams_at_once():
+    """Attention and draws enqueued on two streams without waiting, a workspace each: the results of the calls made one at a time."""
+    L, dtype = wr.load_library(), "bfloat16"
+    rng = np.random.default_rng(8)
+    streams = [L.wmi_dev_stream_create() for _ in range(2)]
+    jobs = []
+    for seed, lens, news in ((31, [9000, 20], [1, 1]), (32, [5000, 700], [60, 200])):
+        cache, hosts, bases, table, q, cu, kv = attn_setup(seed, dtype, lens, news, 2, 4, 128, 16)
+        need = sv.paged_attention_workspace(cache, q.shape[0], q.shape[1], 2, max(news), max(lens))
+        assert need > 0
+        ref = run_attn(cache, table, q, cu, kv, dtype, max(news), max(lens))
+        x, u = dev((rng.standard_normal((40, 20011)) * 2).astype(np.float32)), dev(rng.random(40).astype(np.float32))
+        p, t0, t1 = dev(np.full(40, 0.9, np.float32)), dev(np.zeros(40, np.int32)), dev(np.zeros(40, np.int32))
+        sv.sample_tokens(x, u, t0, top_p=p)
+        jobs.append((cache, bases, dev(q, dtype), dev(table), dev(cu), dev(kv), max(news), max(lens), dev(np.zeros(q.shape, np.uint16), dtype), dev(np.full(need, 0xFF, np.uint8)), ref, x, u, p, t0, t1))
+    assert L.wmi_dev_sync() == 0
+    for _ in range(10):
+        for s, (cache, _, q, table, cu, kv, mn, mk, out, ws, _, x, u, p, _, t1) in zip(streams, jobs):
+            sv.paged_attention(q, cache, table, cu, kv, mn, mk, out, workspace=ws, stream=s)
+            sv.sample_tokens(x, u, t1, top_p=p, stream=s)
+    for s in streams:
+        assert L.wmi_dev_stream_sync(s) == 0
+    for j in jobs:
+        assert np.array_equal(j[8].numpy(), j[10]) and np.array_equal(j[15].numpy(), j[14].numpy())
+    for s in streams:
+        L.wmi_dev_stream_destroy(s)
