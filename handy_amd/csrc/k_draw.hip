@@ -1,6 +1,7 @@
 // One token a row from its logits, for gfx950: temperature, top-k, top-p, min-p, and a draw from a given uniform number.
 #include "kernels.h"
 #include "serving_host.h"
+#include <type_traits>
 
 namespace wmi {
 
@@ -13,15 +14,16 @@ namespace wmi {
 // One workgroup a row; the row comes from HBM once and out of the caches in later passes:
 //   1. the largest value
 //   2. the whole mass (for the log-probability; without a filter also what the draw needs, by wave)
-//   3. the cut. A short top-k or min_p alone: the k-th largest of the threads' own maxima (at least k entries reach it) or the border
+//   3. the cut. A short top-k or a min_p: the k-th largest of the threads' own maxima (at least k entries reach it) or the border
 //      weight bounds it from below; the entries that reach the bound are listed in the LDS, and the rest of the work runs over the list. Other
 //      filters (and lists that overflow): pass 2 also adds counts and masses up in kDrawBins bins of equal width from the largest
 //      value down, masses by wave; the cut lies in the first bin whose running sum reaches what is asked for. Either way that bin's
-//      members are ranked, or resolved by radix selection if there are many.
+//      members are ranked, or narrowed down by radix first if there are many.
 //   4. the draw, in the vocabulary's order: the wave's run that holds it, the thread's few entries, the entry.
 // Bound by 64-bit arithmetic (pass 2: 21 such instructions a weight, about 7 us for 51866 entries on one compute unit) and by the waits
 // of the short steps, which a second row on the same compute unit covers.
 constexpr double kMassOne = 35184372088832.0;               // 2^45
+constexpr float kListMinP = 1.0f / 1024;                    // a min_p from here on is taken to leave few entries
 constexpr int kDrawBins = 768, kDrawRank = 1024, kDrawClose = 128, kDrawCap = 1024;
 
 typedef unsigned long long u64;
@@ -88,7 +90,7 @@ template <int TH> struct DrawShared {
 template <class T, int TH>
 __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
     typedef typename DrawIn<T>::V V4;
-    constexpr int W = TH / 64, U = 4;
+    constexpr int W = TH / 64, U = 4, LOW = sizeof(T) == 4 ? 0 : std::is_same<T, f16>::value ? 13 : 16;      // low bits that a float made from T does not use
     __shared__ DrawShared<TH> sh;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), V = a.n_vocab;
     const T *src = (const T *)a.logits + (a.row_of ? a.row_of[row] : row) * a.row_stride;
@@ -242,48 +244,54 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
     // values. Leaves what it collected of that bin: sh.bin, sh.n_rank, sh.kmin, sh.kmax, sh.n_member, sh.rank*
     auto select = [&](u64 want, bool by_mass, float &v_out, u64 &above_out) __attribute__((always_inline)) {
         auto running = [&](int b) -> u64 { return b < 0 ? 0 : by_mass ? sh.mass[b] : (u64)sh.count[b]; };
-        if (tid == 0) { sh.n_rank = 0; sh.kmin = 0xffffffffu; sh.kmax = 0; }
         for (int i = tid; i < kDrawBins; i += TH) if (running(i) >= want && running(i - 1) < want) sh.bin = i;
         __syncthreads();
         const int bin = sh.bin;
-        const u64 above = running(bin - 1);
-        unsigned members = 0, kmin = 0xffffffffu, kmax = 0;
-        pass([&](float x, int) {
-            if (x != -INFINITY && bin_of(x) == bin) {
-                const unsigned at = atomicAdd(&sh.n_rank, 1u), key = draw_key(x);
-                kmin = min(kmin, key); kmax = max(kmax, key);
-                members++;
-                if (at < (unsigned)kDrawRank) { sh.rank[at] = x; sh.rank_mass[at] = mass_of(x); sh.rank_wave[at] = (unsigned char)wave; }
-            }
-        });
-        for (int o = 32; o > 0; o >>= 1) { members += __shfl_xor(members, o); kmin = min(kmin, (unsigned)__shfl_xor(kmin, o)); kmax = max(kmax, (unsigned)__shfl_xor(kmax, o)); }
-        if (lane == 0 && members) { atomicMin(&sh.kmin, kmin); atomicMax(&sh.kmax, kmax); }
-        if (lane == 0) sh.n_member[wave] = members;
-        __syncthreads();
-        const int n = (int)sh.n_rank;
-        if (sh.kmin == sh.kmax) { v_out = draw_val(sh.kmin); above_out = above; }
-        else if (n <= kDrawRank && narrow(want, by_mass, n, above)) { v_out = sh.cut; above_out = sh.above;
-        } else {                                             // radix selection among the members, 8 bits of the key at a time
-            unsigned prefix = 0;
-            u64 sum = above;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                for (int i = tid; i < 256; i += TH) sh.radix[i] = 0;
-                __syncthreads();
-                pass([&](float x, int) {
-                    const unsigned key = draw_key(x);
-                    if (x != -INFINITY && bin_of(x) == bin && (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))) {
-                        const u64 m = by_mass ? mass_of(x) : 1;
-                        if (m) atomicAdd(&sh.radix[(key >> shift) & 255], m);
-                    }
-                });
-                __syncthreads();
-                pick_digit(want, sum);
-                prefix |= sh.digit << shift;
-                sum = sh.above;
-            }
-            v_out = draw_val(prefix); above_out = sum;
+        u64 above = running(bin - 1);
+        unsigned lo = 0, hi = 0xffffffffu;                   // the keys (without their unused bits) the cut's lies among; the bin's own are an interval
+        bool whole = true;                                   // that is the bin
+        for (;;) {
+            if (tid == 0) { sh.n_rank = 0; sh.kmin = 0xffffffffu; sh.kmax = 0; }
+            __syncthreads();
+            unsigned members = 0, kmin = 0xffffffffu, kmax = 0;
+            pass([&](float x, int) {
+                const unsigned key = draw_key(x);
+                if (x != -INFINITY && (whole ? bin_of(x) == bin : (key >> LOW) - lo <= hi - lo)) {
+                    const unsigned at = atomicAdd(&sh.n_rank, 1u);
+                    kmin = min(kmin, key); kmax = max(kmax, key);
+                    members++;
+                    if (at < (unsigned)kDrawRank) { sh.rank[at] = x; sh.rank_mass[at] = mass_of(x); sh.rank_wave[at] = (unsigned char)wave; }
+                }
+            });
+            for (int o = 32; o > 0; o >>= 1) { members += __shfl_xor(members, o); kmin = min(kmin, (unsigned)__shfl_xor(kmin, o)); kmax = max(kmax, (unsigned)__shfl_xor(kmax, o)); }
+            if (lane == 0 && members) { atomicMin(&sh.kmin, kmin); atomicMax(&sh.kmax, kmax); }
+            if (lane == 0) sh.n_member[wave] = members;
+            __syncthreads();
+            const int n = (int)sh.n_rank;
+            if (sh.kmin == sh.kmax) { v_out = draw_val(sh.kmin); above_out = above; break; }
+            if (n <= kDrawRank && narrow(want, by_mass, n, above)) { v_out = sh.cut; above_out = sh.above; break; }
+            // too many: 256 intervals of equal width of their keys; the one the cut is in
+            lo = sh.kmin >> LOW; hi = sh.kmax >> LOW;
+            const int bits = 32 - __builtin_clz(hi - lo), shift = bits > 8 ? bits - 8 : 0;
+            for (int i = tid; i < 256; i += TH) sh.radix[i] = 0;
+            __syncthreads();
+            pass([&](float x, int) {
+                const unsigned d = (draw_key(x) >> LOW) - lo;
+                if (x != -INFINITY && d <= hi - lo) {
+                    const u64 m = by_mass ? mass_of(x) : 1;
+                    if (m) atomicAdd(&sh.radix[d >> shift], m);
+                }
+            });
+            __syncthreads();
+            pick_digit(want, above);
+            above = sh.above;
+            lo += sh.digit << shift; hi = min(hi, lo + ((1u << shift) - 1));
+            whole = false;
+            if (lo == hi) { v_out = draw_val(lo << LOW | (lo >> (31 - LOW) ? 0 : (1u << LOW) - 1)); above_out = above; break; }
+            __syncthreads();
         }
         __syncthreads();
+        if (!whole) { if (tid == 0) sh.bin = -1; __syncthreads(); }      // (what is collected is not the bin's)
     };
 
     if (top == INFINITY) {                                   // infinite entries share everything: the cut is among them
@@ -303,7 +311,9 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
         if (use_m && min_p > 1.0f) ties = 1;
     } else {
         const bool filtered = !drawn || use_k || use_p || use_m;
-        bool binned = drawn && (use_k ? top_k > TH / 2 : use_p);
+        // min_p bounds the list unless top-p's masses are those of the first top_k, which may reach behind it
+        const bool by_m = use_m && min_p >= kListMinP && !(use_k && use_p);
+        bool binned = drawn && !by_m && (use_k ? top_k > TH / 2 : use_p);
 #pragma clang loop unroll(disable)
         for (;;) {
             if (binned) {
@@ -340,7 +350,7 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
 
             // 3. the list: entries from the bin on that holds the k-th largest of the threads' maxima -- from the lowest maximum in it
             float least = top;
-            if (drawn && !use_k) least = fminf(top, (float)((double)top + T64 * (log(fmin((double)min_p, 1.0)) - 1e-6)));       // (a slack far beyond every rounding here)
+            if (drawn && (by_m || !use_k)) least = fminf(top, (float)((double)top + T64 * (log(fmin((double)min_p, 1.0)) - 1e-6)));       // (a slack far beyond every rounding here)
             else if (drawn) {
                 const unsigned kk = (unsigned)top_k;
                 clear_bins();
@@ -381,7 +391,7 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
 #pragma unroll
             for (int w = 0; w < W; w++) listed &= sh.n_listed[w] <= (unsigned)kDrawCap;
             if (listed) {
-                if (use_k) {
+                if (use_k || use_p) {
                     set_bins(least);
                     clear_bins();
                     __syncthreads();
@@ -431,6 +441,7 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
                 }
                 const double limit = ceil((double)top_p * (double)zk);
                 want = limit > 1.0 ? (u64)limit : 1;
+                if (listed && want > sh.mass[kDrawBins - 1]) break;      // the list ends before: min_p's border decides
             }
             float v;
             u64 above;

@@ -360,6 +360,25 @@ def test_sample_ties_infinities_and_nothing_to_draw(dtype):
         check_sample(x, dtype, u, np.zeros(n), what=("greedy", i))
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("rows,V", [(6, 40000), (6, 5000), (257, 17000)])
+def test_sample_cuts_inside_a_crowd(dtype, rows, V):
+    """Nearly all entries within a few hundredths, one well above: the cut of top-k or top-p lies among thousands of entries that the
+    bins from the largest value down do not tell apart. At positive and negative values, with min_p bounds that leave the crowd in (too
+    many for a list), out, or in part."""
+    rng = np.random.default_rng(V)
+    for shift, gap in ((3.0, 6.0), (-3.0, 6.0), (-0.01, 1.0)):
+        x = shift + 0.01 * rng.standard_normal((rows, V))
+        x[np.arange(rows), rng.integers(0, V, rows)] = shift + gap
+        x = host_form(x, dtype)
+        u = rng.random(rows).astype(np.float32)
+        k, p = rng.integers(V // 10, V, rows), rng.uniform(0.1, 0.95, rows)
+        edge = np.exp(-gap) * rng.uniform(0.98, 1.02, rows)             # weights of the crowd
+        for kk, pp, mm in ((k, None, None), (None, p, None), (k, p, None), (None, p, edge), (k, None, edge), (k, p, edge), (None, p, np.full(rows, 0.9 * np.exp(-gap))),
+                           (None, p, np.full(rows, 0.9)), (None, p, np.full(rows, 1 / 2048)), (np.full(rows, 7), p, np.full(rows, 0.5))):
+            check_sample(x, dtype, u, None, kk, pp, mm, (shift, gap, kk is not None, pp is not None, mm is not None))
+
+
 def test_sample_does_not_depend_on_the_rows_beside():
     rng = np.random.default_rng(12)
     x = (rng.standard_normal((300, 5003)) * 2).astype(np.float32)
