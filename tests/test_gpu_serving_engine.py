@@ -88,6 +88,29 @@ def test_device_draws_repeat_and_differ(wr, model_path):
     st.free(); ctx.free()
 
 
+def test_device_draws_come_after_the_filter(wr, model_path):
+    """What the caller's logits filter removes is never drawn: it leaves one token, then two, and the draws are those."""
+    ctx = wr.WhisperContext(model_path("micro.en", decisive=1.0))
+    pcm = synth_pcm(900, 6 * 16000)
+    seen = set()
+    for keep in ([1234], [1234, 777]):
+        def only(tokens, logits, keep=keep):
+            kept = logits[keep].copy()
+            logits[:] = -np.inf
+            logits[keep] = kept
+        fp = _params(wr, 3)
+        fp.set_no_timestamps(True); fp.set_max_tokens(12); fp.set_filter_logits_callback(only)
+        st = ctx.create_batch_state(1, 4, 1)
+        st.set_device_draws(True)
+        st.full_batch(fp, [pcm])
+        toks = st.batch_tokens(0)
+        assert len(toks) > 0 and set(toks) <= set(keep), toks
+        seen |= set(toks)
+        st.free()
+    assert seen == {1234, 777}
+    ctx.free()
+
+
 def test_window_memo_forgets_when_the_draws_change(wr, model_path):
     """A window remembered under one way of drawing is not taken over under another."""
     ctx = wr.WhisperContext(model_path("micro.en"))
