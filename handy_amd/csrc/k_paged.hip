@@ -610,8 +610,16 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_chunk_kernel(PagedAttn a, At
                 for (int i = 0; i < 16; i++) {
                     const int kk = kh * 32 + (i & 3) + 8 * (i >> 2) + 4 * h, j = k0 + kk;
                     if (j > pos || j < klow) s[kh][i] = -INFINITY;
-                    if (hole && bad_flag[buf][(kk / RPI) % WV] && bad_key[buf][kk]) s[kh][i] = -INFINITY;
                 }
+            if (hole) {
+#pragma unroll
+                for (int kh = 0; kh < 2; kh++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int kk = kh * 32 + (i & 3) + 8 * (i >> 2) + 4 * h;
+                        if (bad_flag[buf][(kk / RPI) % WV] && bad_key[buf][kk]) s[kh][i] = -INFINITY;
+                    }
+            }
         }
         float mx = -INFINITY;
 #pragma unroll
