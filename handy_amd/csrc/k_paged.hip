@@ -134,7 +134,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
 //   paged_step_kernel    up to 16 packed rows (single tokens): bound by HBM. Each wave streams its own 16-key tiles. 64 requests of up
 //                        to 8192 keys, 32/8 heads x 128, bf16: 182 us, 6.3 TB/s; 3 of 90 000 - 131 000 keys: 216 us, 6.7 TB/s.
 //   paged_chunk_kernel   128 or 256 packed rows a workgroup, 64-key tiles shared by its waves. Three chunks of about 3800 tokens behind
-//                        20 000 - 28 500 cached ones, 32/8 heads x 128, bf16: 5.2 ms, 1035 TFLOP/s; bound by issue: the matrix pipes are
+//                        20 000 - 28 500 cached ones, 32/8 heads x 128, bf16: 5.2 ms, 1030 TFLOP/s; bound by issue: the matrix pipes are
 //                        busy 44 % of the CU cycles, the vector instructions between two products (exponentials, conversions, the
 //                        running maximum) fill the rest. Prompts of up to 224 tokens, 64 x 20 heads x 64, f16: 33 us, bound by the chain
 //                        lengths - table - keys - two to four tiles in each short-lived workgroup.
@@ -194,14 +194,15 @@ __device__ __attribute__((aligned(16))) unsigned attn_zero_chunk[4];     // what
 
 struct AttnReq { int q0, n, len; };
 // lengths and offsets of a request, forced into the call's buffers whatever the arrays hold
-__device__ __forceinline__ AttnReq attn_req(const PagedAttn &a, int i) {
+__device__ __forceinline__ AttnReq attn_req(const PagedAttn &a, int cu0, int cu1, int kv_len) {
     AttnReq r;
-    r.q0 = min(max(a.cu[i], 0), a.n_rows);
-    r.n = min(max(a.cu[i + 1], r.q0), a.n_rows) - r.q0;
+    r.q0 = min(max(cu0, 0), a.n_rows);
+    r.n = min(max(cu1, r.q0), a.n_rows) - r.q0;
     const long room = (long)a.cols << a.lp;
-    r.len = (int)min((long)max(a.kv_lens[i], 0), min(room, 0x7fffffffL));
+    r.len = (int)min((long)max(kv_len, 0), min(room, 0x7fffffffL));
     return r;
 }
+__device__ __forceinline__ AttnReq attn_req(const PagedAttn &a, int i) { return attn_req(a, a.cu[i], a.cu[i + 1], a.kv_lens[i]); }
 // keys [lo, hi) that the packed rows r0 .. r1 - 1 of a request see between them
 __device__ __forceinline__ void attn_keys(const PagedAttn &a, const AttnReq &q, int r0, int r1, int &lo, int &hi) {
     const int first = q.len - q.n + r0 / a.group, last = q.len - q.n + (r1 - 1) / a.group;
@@ -478,16 +479,19 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_chunk_kernel(PagedAttn a, At
     const int nblk = gridDim.x, xq = nblk >> 3, xr = nblk & 7, xcd = blockIdx.x & 7, xi = blockIdx.x >> 3;
     const int logical = (xcd < xr ? xcd * (xq + 1) : xr * (xq + 1) + (xcd - xr) * xq) + xi;
     const int part = logical % ps.splits, tile = n_tiles - 1 - (logical / ps.splits) % n_tiles, head = logical / ps.splits / n_tiles;
-    int req = 0;
-    for (int left = a.n_seq; left > 1;) {                                  // the last request whose first tile number is <= tile, 64 ways at a time
-        const int step = (left + 63) / 64, i = req + lane * step;
-        const bool ok = lane * step < left && (long)a.cu[i] * a.group / ROWS + i <= tile;
-        const int k = max(__popcll(__ballot(ok)) - 1, 0);
+    int req = 0, cu0, cu1, kv_len;
+    for (int left = a.n_seq;;) {                                           // the last request whose first tile number is <= tile, 64 ways at a time
+        const int step = (left + 63) / 64, i = min(req + lane * step, a.n_seq - 1), c0 = a.cu[i], c1 = a.cu[i + 1], kv = a.kv_lens[i];
+        const bool ok = lane * step < left && (long)c0 * a.group / ROWS + i <= tile;
+        const int k = __builtin_amdgcn_readfirstlane(max(__popcll(__ballot(ok)) - 1, 0));
         req += k * step; left = min(step, left - k * step);
+        if (step == 1) {                                                   // its lane has what the request is (a round trip less before the first loads)
+            cu0 = __builtin_amdgcn_readlane(c0, k); cu1 = __builtin_amdgcn_readlane(c1, k); kv_len = __builtin_amdgcn_readlane(kv, k);
+            break;
+        }
     }
-    req = __builtin_amdgcn_readfirstlane(req);
-    const AttnReq rq = attn_req(a, req);
-    const long r0l = ((long)tile - ((long)a.cu[req] * a.group / ROWS + req)) * ROWS;
+    const AttnReq rq = attn_req(a, cu0, cu1, kv_len);
+    const long r0l = ((long)tile - ((long)cu0 * a.group / ROWS + req)) * ROWS;
     const int rows = rq.n * a.group;
     if (r0l < 0 || r0l >= rows) return;
     const int r0 = (int)r0l, r1 = min(rows, r0 + ROWS);
