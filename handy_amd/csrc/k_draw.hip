@@ -20,7 +20,7 @@ namespace wmi {
 //      value down, masses by wave; the cut lies in the first bin whose running sum reaches what is asked for. Either way that bin's
 //      members are ranked, or narrowed down by radix first if there are many.
 //   4. the draw, in the vocabulary's order: the wave's run that holds it, the thread's few entries, the entry.
-// Bound by 64-bit arithmetic (pass 2: 21 such instructions a weight, about 7 of its 11 us for 51866 entries on one compute unit) and by
+// Bound by 64-bit arithmetic (pass 2: 19 such instructions a weight, about 7 of its 11 us for 51866 entries on one compute unit) and by
 // the waits of the short steps, which a second row on the same compute unit covers. Five rows of 51866 32-bit logits at a temperature:
 // 25 us; 1024 rows with every filter in use: 150 us (1.4 TB/s of logits); 48 rows of 131071 bf16: 95 us.
 constexpr double kMassOne = 35184372088832.0;               // 2^45
@@ -58,8 +58,7 @@ struct DrawScale {
         return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
     }
     // rounded to a multiple of 2^-45: 128 plus the weight keeps 45 bits behind the point, and is that whole number but for its exponent
-    __device__ __forceinline__ double rounded(float x) const { return exact(x) + 128.0; }
-    __device__ __forceinline__ u64 mass(float x) const { return (u64)__double_as_longlong(rounded(x)) - 0x4060000000000000ull; }
+    __device__ __forceinline__ u64 mass(float x) const { return (u64)__double_as_longlong(exact(x) + 128.0) - 0x4060000000000000ull; }
 };
 
 template <class T> struct DrawIn;                            // four consecutive logits at any alignment
@@ -325,23 +324,22 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
                 __syncthreads();
             }
             // 2. the whole mass
-            double acc = 0.0;                                // at most 256 multiples of 2^-45 up to 1: exact
+            u64 own = 0;
             if (!binned) stream4([&](const float *v, int) {
 #pragma unroll
-                for (int c = 0; c < 4; c++) acc += sc.rounded(v[c]) - 128.0;
+                for (int c = 0; c < 4; c++) own += sc.mass(v[c]);
             });
             else stream4([&](const float *v, int) {
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    const double r = sc.rounded(v[c]);
-                    const u64 m = (u64)__double_as_longlong(r) - 0x4060000000000000ull;
+                    const u64 m = sc.mass(v[c]);
                     const int b = bin_of(v[c]);
-                    acc += r - 128.0;
+                    own += m;
                     if (use_k && v[c] != -INFINITY) atomicAdd(&sh.count[b], 1u);
                     if (m) atomicAdd(&sh.hist[wave][b], m);
                 }
             });
-            const u64 own = wave_sum64((u64)(acc * kMassOne));
+            own = wave_sum64(own);
             if (lane == 0) { sh.seg_mass[wave] = own; sh.seg_ties[wave] = 0; }
             __syncthreads();
             z = 0;
@@ -574,7 +572,7 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
 template <class T> static void draw_launch(const DrawArgs &a, hipStream_t st) {
     // Short rows: four waves a row, so that more rows share a compute unit. Else sixteen if every row has a compute unit of its own
     // (256), or eight, two rows a compute unit, whose waits then fall under the other's arithmetic (1024 rows of 51866 entries: 99 us
-    // against 125). Rows past 131072 always take sixteen: a thread's sum of masses is exact for 256 entries.
+    // against 125). Longer rows take sixteen again: a thread's share is long enough (600 rows of 262144: 317 us against 360).
     if (a.n_vocab <= 16384) hipLaunchKernelGGL((draw_kernel<T, 256>), dim3(a.n_rows), dim3(256), 0, st, a);
     else if (a.n_rows > 256 && a.n_vocab <= 131072) hipLaunchKernelGGL((draw_kernel<T, 512>), dim3(a.n_rows), dim3(512), 0, st, a);
     else hipLaunchKernelGGL((draw_kernel<T, 1024>), dim3(a.n_rows), dim3(1024), 0, st, a);

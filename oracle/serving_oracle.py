@@ -1,5 +1,5 @@
 """Plain restatement in numpy (64-bit) of the serving operators of include/wmi.h: wmi_paged_plan, wmi_paged_write,
-wmi_paged_attention, wmi_sample_tokens. The checker of tests/test_gpu_serving.py and tests/test_cpu_serving.py only."""
+wmi_paged_attention, wmi_sample_tokens. What tests/test_gpu_serving.py and tests/test_cpu_serving.py compare with, used there only."""
 import numpy as np
 
 
