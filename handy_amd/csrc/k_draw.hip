@@ -260,7 +260,7 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
                     const unsigned at = atomicAdd(&sh.n_rank, 1u);
                     kmin = min(kmin, key); kmax = max(kmax, key);
                     members++;
-                    if (at < (unsigned)kDrawRank) { sh.rank[at] = x; sh.rank_mass[at] = mass_of(x); sh.rank_wave[at] = (unsigned char)wave; }
+                    if (at < (unsigned)kDrawRank) { sh.rank[at] = x; sh.rank_wave[at] = (unsigned char)wave; }
                 }
             });
             for (int o = 32; o > 0; o >>= 1) { members += __shfl_xor(members, o); kmin = min(kmin, (unsigned)__shfl_xor(kmin, o)); kmax = max(kmax, (unsigned)__shfl_xor(kmax, o)); }
@@ -268,6 +268,10 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
             if (lane == 0) sh.n_member[wave] = members;
             __syncthreads();
             const int n = (int)sh.n_rank;
+            if (n <= kDrawRank) {                            // (their masses here, not in the pass, where one member costs its whole wave the arithmetic)
+                for (int i = tid; i < n; i += TH) sh.rank_mass[i] = mass_of(sh.rank[i]);
+                __syncthreads();
+            }
             if (sh.kmin == sh.kmax) { v_out = draw_val(sh.kmin); above_out = above; break; }
             if (n <= kDrawRank && narrow(want, by_mass, n, above)) { v_out = sh.cut; above_out = sh.above; break; }
             // too many: 256 intervals of equal width of their keys; the one the cut is in
@@ -278,16 +282,21 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
             pass([&](float x, int) {
                 const unsigned d = (draw_key(x) >> LOW) - lo;
                 if (x != -INFINITY && d <= hi - lo) {
-                    const u64 m = by_mass ? mass_of(x) : 1;
+                    const u64 m = by_mass && shift > 0 ? mass_of(x) : 1;
                     if (m) atomicAdd(&sh.radix[d >> shift], m);
                 }
             });
             __syncthreads();
+            auto value_of = [&](unsigned key) { return draw_val(key << LOW | (key >> (31 - LOW) ? 0 : (1u << LOW) - 1)); };
+            if (by_mass && shift == 0) {                     // every interval is one value: counted
+                for (int i = tid; i <= (int)(hi - lo); i += TH) sh.radix[i] *= mass_of(value_of(lo + i));
+                __syncthreads();
+            }
             pick_digit(want, above);
             above = sh.above;
             lo += sh.digit << shift; hi = min(hi, lo + ((1u << shift) - 1));
             whole = false;
-            if (lo == hi) { v_out = draw_val(lo << LOW | (lo >> (31 - LOW) ? 0 : (1u << LOW) - 1)); above_out = above; break; }
+            if (lo == hi) { v_out = value_of(lo); above_out = above; break; }
             __syncthreads();
         }
         __syncthreads();
