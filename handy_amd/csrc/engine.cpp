@@ -1391,7 +1391,10 @@ int Engine::Run::run_group(const float *const *pcm, const int *n, int g0, int G,
             for (int c = 0; c < 8; c++) d.topk[c] = tk[lr * 8 + c];
             if (srows[lr].want_probs == 1) d.probs.assign(E.probs_host_.as<float>() + lr * (size_t)E.V_, E.probs_host_.as<float>() + (lr + 1) * (size_t)E.V_);
         }
-        for (size_t i = 0; i < draws.size(); i++) { Decoder &d = utts[draw_ref[i].utt].dec[draw_ref[i].dec]; d.draw_id = draws[i].id >= 0 ? draws[i].id : d.so.id; d.draw_plog = draws[i].plog; }   // (-1: the rules left nothing)
+        for (size_t i = 0; i < draws.size(); i++) {           // (-1: the rules left nothing; then the selection of the row the draw looked at)
+            Decoder &d = utts[draw_ref[i].utt].dec[draw_ref[i].dec];
+            d.draw_id = draws[i].id >= 0 ? draws[i].id : so[draws[i].logit_row].id; d.draw_plog = draws[i].plog;
+        }
         // ---- advance the state machines of the utterances that were in the pass
         for (int i = 0; i < G; i++) {
             Utt &u = utts[i];

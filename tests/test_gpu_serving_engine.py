@@ -217,3 +217,29 @@ def test_prompt_attention_transcripts_match_the_oracle(wr, oracle, model_path, a
         assert st.batch_tokens(u) == ref and one.batch_tokens(0) == ref and len(ref) > 0
         one.free(); o.close()
     st.free(); ctx.free(); om.close()
+
+
+def test_device_draws_where_nothing_is_left_take_the_rows_own_token(wr, model_path):
+    """A caller's filter that leaves nothing on the prompt row of the second window: every one of the best-of-three decoders starts with what that
+    row selects (id 0), none with the token it had selected last in the window before."""
+    ctx = wr.WhisperContext(model_path("micro.en", decisive=1.0))
+    prompts, starts = [0], {1: set(), 2: set()}
+
+    def only(tokens, logits):
+        if not tokens:
+            prompts[0] += 1
+            if prompts[0] == 2:
+                logits[:] = -np.inf
+                return
+        else:
+            starts[prompts[0]].add(tokens[0].id)
+        kept = logits[777].copy()
+        logits[:] = -np.inf
+        logits[777] = kept
+    fp = _params(wr, 3)
+    fp.set_no_timestamps(True); fp.set_max_tokens(6); fp.set_filter_logits_callback(only)
+    st = ctx.create_batch_state(1, 4, 1)
+    st.set_device_draws(True)
+    st.full_batch(fp, [synth_pcm(900, 45 * 16000)])
+    assert prompts[0] == 2 and starts == {1: {777}, 2: {0}}, (prompts, starts)
+    st.free(); ctx.free()
