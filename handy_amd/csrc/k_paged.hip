@@ -139,8 +139,12 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
 //                        running maximum) fill the rest. Prompts of up to 224 tokens, 64 x 20 heads x 64, f16: 33 us, bound by the chain
 //                        lengths - table - keys - two to four tiles in each short-lived workgroup.
 // The keys of a tile of rows may be split over workgroups; paged_join_kernel adds the parts up.
-// The reference exponent of a row moves only when a score passes it by more than 8 (in powers of two): probabilities stay below
-// 2^8, which both 16-bit types hold at full relative precision, and the accumulators are rescaled rarely instead of every tile.
+// The reference exponent of a row moves only when a score passes it by more than kMove (in powers of two), so that the accumulators
+// are rescaled rarely instead of every tile. Probabilities are 2^(score - reference + kBias), rounded to the cache's type for the product
+// with V (their sums are of the unrounded ones); the factor 2^kBias cancels against the sum. bf16 holds them at 8 bits whatever their size.
+// f16 does not: its 15 powers of two above 1 are used up (4 + 11), so that weights down to 2^-25 of the reference's keep 11 bits and those
+// down to 2^-36 fewer -- without the bias a long tail behind one key 17 nats above it came out 44 % too large.
+// (Chunks of 4096, f16, 128 dims: 5.82 ms with 4 + 11, 5.74 with 8 + 7, 5.90 with 2 + 13; single tokens and 64 dims do not tell them apart.)
 typedef __bf16 bf16;
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -152,6 +156,7 @@ template <class T> struct Mma;
 template <> struct Mma<f16> {
     typedef f16x8 V8; typedef f16x4 V4;
     static constexpr unsigned short kExp = 0x7c00, kOne = 0x3c00, kSign = 0x8000;
+    static constexpr float kMove = 4.0f, kBias = 11.0f;
     static __device__ __forceinline__ f32x16 m32(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x4 m16k32(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x4 m16k16(V4 a, V4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
@@ -159,6 +164,7 @@ template <> struct Mma<f16> {
 template <> struct Mma<bf16> {
     typedef bf16x8 V8; typedef bf16x4 V4;
     static constexpr unsigned short kExp = 0x7f80, kOne = 0x3f80, kSign = 0x8000;
+    static constexpr float kMove = 8.0f, kBias = 0.0f;
     static __device__ __forceinline__ f32x16 m32(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x4 m16k32(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x4 m16k16(V4 a, V4 b, f32x4 c) {
@@ -215,7 +221,6 @@ __device__ __forceinline__ int attn_parts(int n_kt, int splits, int least) { ret
 constexpr int kStepRows = 16, kStepKeys = 16, kChunkKeys = 64;
 constexpr int kStepLeast = 32, kChunkLeast = 4;        // shortest part, in key tiles (512 and 256 keys): below that the join costs more than it saves
 constexpr int kMaxParts = 256;                         // the join gives every part a thread
-constexpr float kMoveBy = 8.0f;
 
 // partial results of a split call: [part][row][query head][DP] accumulators, then {reference exponent, sum}
 struct AttnParts { float *o; float2 *ml; int splits; };
@@ -336,7 +341,7 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(PagedAttn a, AttnPar
                 }
             }
             const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) * c;
-            if (__any(mx > m + kMoveBy)) {
+            if (__any(mx > m + M::kMove)) {
                 float mn = fmaxf(mx, __shfl_xor(mx, 16));
                 mn = fmaxf(fmaxf(mn, __shfl_xor(mn, 32)), m);
                 const float al = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -345,7 +350,7 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(PagedAttn a, AttnPar
                 for (int i = 0; i < NB; i++) o[i] *= al;
                 m = mn;
             }
-            const float mu = m == -INFINITY ? 0.0f : m;
+            const float mu = m == -INFINITY ? 0.0f : m - M::kBias;
             V4 p;
 #pragma unroll
             for (int r = 0; r < 4; r++) { const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -mu)); l += e; p[r] = (T)e; }
@@ -631,14 +636,14 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_chunk_kernel(PagedAttn a, At
 #pragma unroll
             for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[kh][i]);
         mx *= c;
-        if (__any(mx > m + kMoveBy)) {
+        if (__any(mx > m + M::kMove)) {
             const float mn = fmaxf(fmaxf(mx, __shfl_xor(mx, 32)), m), al = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
             l *= al;
 #pragma unroll
             for (int b = 0; b < NB; b++) o[b] *= al;
             m = mn;
         }
-        const float mu = m == -INFINITY ? 0.0f : m;
+        const float mu = m == -INFINITY ? 0.0f : m - M::kBias;
         V8 p[4];
 #pragma unroll
         for (int kh = 0; kh < 2; kh++)

@@ -304,7 +304,8 @@ WHISPER_API int wmi_paged_write(const wmi_paged_cache *cache, const void *k_new,
  * cu_q[n_seq] are left as they are. out shares no memory with what is read. head_dim a multiple of 8 up to 128; 16-byte aligned pointers, strides multiples of 8.
  * max_new and max_kv: the longest request's new and total tokens, as far as the caller knows (they steer how the work is split,
  * larger or smaller values change no result beyond rounding; 0: not known). Scores, softmax and sums are 32-bit; the
- * probabilities are rounded to the cache's type for the product with V. An infinite V may come out as NaN in the rows that see it. */
+ * probabilities are rounded to the cache's type for the product with V (F16: those under 2^-25 of a row's largest keep fewer than 11
+ * bits, those under 2^-36 none). An infinite V may come out as NaN in the rows that see it. */
 typedef struct wmi_paged_attn {
     const void *q;             /* [n_rows][n_q_heads][head_dim], the cache's type */
     void *out;                 /* the same shape and type */

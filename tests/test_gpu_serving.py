@@ -598,3 +598,31 @@ def test_calls_on_two_streams_at_once():
         assert np.array_equal(j[8].numpy(), j[10]) and np.array_equal(j[15].numpy(), j[14].numpy())
     for s in streams:
         L.wmi_dev_stream_destroy(s)
+
+
+# ------------------------------------------------------------------------------------------------ attention: long tails
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("n,dim,page", [(131071, 64, 64), (40000, 128, 16)])
+@pytest.mark.parametrize("new,sink", [(1, "first"), (1, "last"), (40, "first")])
+def test_attention_keeps_a_long_tail_behind_one_key(dtype, n, dim, page, new, sink):
+    """One key whose score is far above all others' and whose V is 0: the result is the others', each a tiny weight. Bound: check_attn's, plus
+    what a 16-bit probability below its normal numbers loses, half a step of 2^-24 against the 2^11 that the largest of a row is held at
+    (float16; bfloat16 has no such numbers here), for every key: n 2^-36 of the largest |v|."""
+    rng = np.random.default_rng(n + dim)
+    n_pages = -(-n // page)
+    at = 0 if sink == "first" else n - 1
+    for gap in (15.0, 16.0, 17.0, 17.4, 19.0):
+        k = 0.02 * rng.standard_normal((n_pages * page, 1, dim))
+        v = rng.uniform(0.5, 1.5, (n_pages * page, 1, dim))
+        k[at], v[at] = gap / dim ** 0.5, 0.0
+        hosts = [host_form(x.reshape(n_pages, page, 1, dim), dtype) for x in (k, v)]
+        cache = sv.PagedCache(*(dev(h, dtype) for h in hosts))
+        table, cu, kv = np.arange(n_pages, dtype=np.int32)[None], np.array([0, new], np.int32), np.array([n], np.int32)
+        q = host_form(np.ones((new, 2, dim)), dtype)
+        ref, mass, reach = so.attention(values(q, dtype), values(hosts[0], dtype), values(hosts[1], dtype), table, cu, kv, page, dim ** -0.5)
+        half = HALF_STEP[dtype]
+        rel = 2 * half + 2 * (dim + 8) * 2.0 ** -24 * reach[:, :, None] + 2 * n * 2.0 ** -24 + 2.0 ** -20
+        tol = half * np.abs(ref) + rel * mass * 1.01 + (2.0 ** -24 + n * 2.0 ** -36 * 1.5 if dtype == "float16" else 2.0 ** -126)
+        for hint in (n, 1):                                        # keys split over workgroups, and all of them in one
+            got = values(run_attn(cache, table, q, cu, kv, dtype, new, hint), dtype)
+            assert (np.abs(got - ref) <= tol).all(), (gap, hint, float((np.abs(got - ref) / tol).max()), got.flat[0], ref.flat[0])
