@@ -126,6 +126,8 @@ def _table(x, n_seq: int):
     if len(s) != 2 or s[0] != n_seq or _dtype(x) != "int32" or (st[1] != 1 and s[1] > 1):
         raise ValueError("block_table: expected int32 [n_seq, cols] with contiguous rows")
     cols = s[1]
+    if n_seq > 1 and st[0] < cols:
+        raise ValueError("block_table: its rows share memory (an expanded row, or overlapping ones)")
     return x.data_ptr() if n_seq and cols else None, max(st[0], cols), cols
 
 

@@ -167,3 +167,22 @@ def test_numbers_out_of_range_are_value_errors():
             sv.paged_attention(q, cache, i32(3, 8), i32(4), i32(3), 1, 100, out, **kw)
     with pytest.raises(ValueError):
         sv.paged_attention(q, cache, i32(3, 8), i32(4), i32(3), 1, 2 ** 33, out)
+
+
+def test_tables_whose_rows_share_memory_are_refused():
+    """A table expanded from one row (stride 0) or with overlapping rows owns fewer entries than rows times columns: no stride of the library's
+    own choice may reach past them. A single row's stride does not matter."""
+    cache = sv.PagedCache(Fake((8, 16, 2, 64), "float16"), Fake((8, 16, 2, 64), "float16"))
+    i32 = lambda *s: Fake(s, "int32")
+    plan = sv.PagePlan(i32(4), i32(3), i32(9), i32(9), i32(4))
+    for stride in (0, 1, 7):
+        table = Fake((3, 8), "int32", (stride, 1))
+        with pytest.raises(ValueError, match="share memory"):
+            sv._table(table, 3)
+        with pytest.raises(ValueError, match="share memory"):
+            sv.plan_pages(i32(3), i32(3), i32(5), table, 16, plan)
+        with pytest.raises(ValueError, match="share memory"):
+            sv.paged_attention(Fake((5, 4, 64), "float16"), cache, table, i32(4), i32(3), 1, 100, Fake((5, 4, 64), "float16", ptr=0x90000))
+        assert sv._table(Fake((1, 8), "int32", (stride, 1)), 1) == (0x10000, 8, 8)
+    assert sv._table(Fake((3, 8), "int32", (11, 1)), 3) == (0x10000, 11, 8)
+    assert sv._table(Fake((3, 0), "int32", (0, 1)), 3)[1:] == (0, 0)
