@@ -72,14 +72,15 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
     for (int i = F + tid; i <= B; i += blockDim.x) { tok[i] = n_tok; pag[i] = n_pag; }
     __syncthreads();
 
-    const int gtid = blockIdx.x * blockDim.x + tid, gsize = gridDim.x * blockDim.x;
+    const unsigned gtid = blockIdx.x * blockDim.x + tid, gsize = gridDim.x * blockDim.x;        // (unsigned: a stride past the last of 2^31 - 1 rows must not wrap)
     // the last request whose sum is <= x among those that own anything: upper bound minus one
     auto owner = [&](const int *s, int x) { int lo = 0, hi = B; while (lo < hi) { const int m = (lo + hi) >> 1; if (s[m + 1] <= x) lo = m + 1; else hi = m; } return lo; };
-    for (int x = gtid; x < n_pag; x += gsize) {
-        const int i = owner(pag, x);
+    for (unsigned w = gtid; w < (unsigned)n_pag; w += gsize) {
+        const int x = (int)w, i = owner(pag, x);
         a.table[i * a.table_stride + ((a.ctx[i] + P - 1) >> a.lp) + (x - pag[i])] = a.free_pages[x];
     }
-    for (int x = gtid; x < a.cap; x += gsize) {
+    for (unsigned w = gtid; w < (unsigned)a.cap; w += gsize) {
+        const int x = (int)w;
         int slot = -1, pos = 0;
         if (x < n_tok) {
             const int i = owner(tok, x), c = a.ctx[i], first = (c + P - 1) >> a.lp;
@@ -92,7 +93,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
         a.slots[x] = slot;
         a.positions[x] = pos;
     }
-    for (int i = gtid; i <= B; i += gsize) {
+    for (int i = (int)gtid; i <= B; i += (int)gsize) {
         a.cu[i] = tok[i];
         if (i < B) { long long n, p; const bool ok = lengths(i, n, p); a.kv[i] = ok ? a.ctx[i] + (i < F ? (int)n : 0) : 0; }
     }
@@ -867,7 +868,7 @@ WHISPER_API int wmi_paged_plan(const int *ctx_lens, const int *new_lens, int n_s
     if (lds > 48 * 1024 && hipFuncSetAttribute((const void *)paged_plan_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) { (void)hipGetLastError(); return -4; }
     // rows beyond two a thread are spread over workgroups, one a CU at most, each of which repeats the prefix sum (4096 requests and 303 000
     // rows, the whole call: 11.8 us with 2048 rows a workgroup, 12.0 with 1024, 14.0 with 4096)
-    const int want = (n_rows_cap + 2047) / 2048, groups = want < 1 ? 1 : want > 256 ? 256 : want;
+    const int want = n_rows_cap / 2048 + (n_rows_cap % 2048 != 0), groups = want < 1 ? 1 : want > 256 ? 256 : want;
     hipLaunchKernelGGL(paged_plan_kernel, dim3(groups), dim3(kPlanThreads), lds, st, a);
     return serve_done();
 }

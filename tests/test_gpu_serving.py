@@ -626,3 +626,32 @@ def test_attention_keeps_a_long_tail_behind_one_key(dtype, n, dim, page, new, si
         for hint in (n, 1):                                        # keys split over workgroups, and all of them in one
             got = values(run_attn(cache, table, q, cu, kv, dtype, new, hint), dtype)
             assert (np.abs(got - ref) <= tol).all(), (gap, hint, float((np.abs(got - ref) / tol).max()), got.flat[0], ref.flat[0])
+
+
+# ------------------------------------------------------------------------------------------------ plan: the largest row count
+def test_plan_of_two_to_the_31_rows():
+    """n_rows_cap = 2^31 - 1, the largest the entry takes (8.6 GB each of slots and positions): the rows at both ends are planned, and what lies in
+    front of the two arrays and behind them is left alone."""
+    L, cap, guard = wr.load_library(), 2 ** 31 - 1, 4096
+    arrays = [sv.DeviceArray(cap + 2 * guard, "int32") for _ in range(2)]
+    mark = np.full(guard, 0x5A5A5A5A, np.int32)
+    for a in arrays:
+        for at in (0, guard + cap):
+            assert L.wmi_dev_upload(a.data_ptr() + 4 * at, mark.ctypes.data, mark.nbytes) == 0
+    ctx, new, free, page, cols = [5, 30], [40, 1], np.arange(7, 17, dtype=np.int32), 16, 4
+    table = np.array([[0, -1, -1, -1], [1, 2, -1, -1]], np.int32)
+    out = sv.PagePlan(dev(np.zeros(3, np.int32)), dev(np.zeros(2, np.int32)), arrays[0].view((cap,), (1,), guard), arrays[1].view((cap,), (1,), guard), dev(np.zeros(4, np.int32)))
+    td = dev(table)
+    sv.plan_pages(dev(np.array(ctx, np.int32)), dev(np.array(new, np.int32)), dev(free), td, page, out)
+    assert L.wmi_dev_sync() == 0
+    ref = so.plan(ctx, new, free, page, table, 4096)
+    for g, r in zip((td, out.cu_q, out.kv_lens, out.counts), (ref[0], ref[1], ref[2], ref[5])):
+        assert np.array_equal(g.numpy(), r)
+    got = np.empty(4096, np.int32)
+    for a, first, rest in zip(arrays, ref[3:5], (-1, 0)):
+        for at in (0, 2 ** 30, cap - 4096):
+            assert L.wmi_dev_download(got.ctypes.data, a.data_ptr() + 4 * (guard + at), got.nbytes) == 0
+            assert np.array_equal(got, first if at == 0 else np.full(4096, rest)), at
+        for at in (0, guard + cap):
+            assert L.wmi_dev_download(got.ctypes.data, a.data_ptr() + 4 * at, got.nbytes) == 0 and np.array_equal(got, mark), at
+        a.free()
