@@ -140,12 +140,14 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
 //                        running maximum) fill the rest. Prompts of up to 224 tokens, 64 x 20 heads x 64, f16: 33 us, bound by the chain
 //                        lengths - table - keys - two to four tiles in each short-lived workgroup.
 // The keys of a tile of rows may be split over workgroups; paged_join_kernel adds the parts up.
-// The reference exponent of a row moves only when a score passes it by more than kMove (in powers of two), so that the accumulators
-// are rescaled rarely instead of every tile. Probabilities are 2^(score - reference + kBias), rounded to the cache's type for the product
-// with V (their sums are of the unrounded ones); the factor 2^kBias cancels against the sum. bf16 holds them at 8 bits whatever their size.
-// f16 does not: its 15 powers of two above 1 are used up (4 + 11), so that weights down to 2^-25 of the reference's keep 11 bits and those
-// down to 2^-36 fewer -- without the bias a long tail behind one key 17 nats above it came out 44 % too large.
-// (Chunks of 4096, f16, 128 dims: 5.82 ms with 4 + 11, 5.74 with 8 + 7, 5.90 with 2 + 13; single tokens and 64 dims do not tell them apart.)
+// A probability is 2^(score c - m), c = |scale| log2(e); its row's reference m moves only when a score passes m + kBias by more than kMove, so
+// that the accumulators are rescaled rarely instead of every tile. m is a whole number: rescaling and joining multiply by powers of two, and a
+// probability's rounding to the cache's type (for the product with V; the sums are of the unrounded ones) does not depend on where its
+// row's reference lies. kBias puts f16's range above 1 to use: the largest probability of a row lies near 2^11 and none reaches 2^16, so
+// that weights down to 2^-25 of the largest keep 11 bits and those down to 2^-36 fewer (with kBias 0 a long tail behind one key 17 nats
+// above it came out 44 % too large). bf16 holds 8 bits whatever the size.
+// (Chunks of 4096, f16, 128 dims: 5.82 ms with kMove + kBias = 4 + 11, 5.74 with 8 + 7, 5.90 with 2 + 13; single tokens and 64 dims do not tell
+// them apart.)
 typedef __bf16 bf16;
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -226,6 +228,25 @@ constexpr int kMaxParts = 256;                         // the join gives every p
 // partial results of a split call: [part][row][query head][DP] accumulators, then {reference exponent, sum}
 struct AttnParts { float *o; float2 *ml; int splits; };
 
+// A row's reference while its keys go by. Where score * c is 2^20 or more, the rounded product that a reference is made of and the fma in
+// the exponent part by a tenth of a power of two and more (from 2^28 on by more than the type's range: finite scores gave NaN, or zeros).
+// Such a row takes its largest score off first, which leaves the largest ones exact; the products then only scale what is summed up already.
+template <class T> struct AttnRef {
+    float limit = -INFINITY;                               // scores above it move the reference (-infinity: none seen)
+    float sub = 0.0f, base = 0.0f;                         // exponents are (score - base) c - sub; base 0: sub is the reference
+    __device__ __forceinline__ float at(float c) const { return limit == -INFINITY ? limit : base != 0.0f ? base * c - Mma<T>::kBias : sub; }
+    // to the largest score `top` if it passes the limit; the factor for what has been summed up
+    __device__ __forceinline__ float move(float top, float c) {
+        if (!(top > limit)) return 1.0f;
+        const float was = at(c), mx = top * c;
+        const bool big = fabsf(mx) >= 0x1p20f;
+        base = big ? top : 0.0f;
+        sub = (big ? 0.0f : ceilf(mx)) - Mma<T>::kBias;
+        limit = big ? top : (sub + (Mma<T>::kBias + Mma<T>::kMove)) / c;
+        return __builtin_amdgcn_exp2f(was - at(c));
+    }
+};
+
 template <class T> __device__ __forceinline__ u16x4 not_finite(typename Mma<T>::V4 v) {
     const u16x4 b = __builtin_bit_cast(u16x4, v);
     return (u16x4)((b & Mma<T>::kExp) == Mma<T>::kExp);                    // all ones where infinite or NaN
@@ -286,7 +307,9 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(PagedAttn a, AttnPar
         f32x4 o[NB];
 #pragma unroll
         for (int i = 0; i < NB; i++) o[i] = f32x4{0, 0, 0, 0};
-        float m = -INFINITY, l = 0.0f;
+        AttnRef<T> ref;
+        bool shift = false;                                                // some row's scores are too large to do without base
+        float l = 0.0f;
         int pg[PAGE16 ? 1 : NI];
         // table entries: PAGE16 -- lane x holds the entry of this wave's tile number (base + x); else one entry per load and lane
         auto entries = [&](int t) {
@@ -341,20 +364,21 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(PagedAttn a, AttnPar
                     if (j > pos || j < klow || j < lo || j >= hi || ((bad_keys >> kk) & 1)) s[r] = -INFINITY;
                 }
             }
-            const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) * c;
-            if (__any(mx > m + M::kMove)) {
-                float mn = fmaxf(mx, __shfl_xor(mx, 16));
-                mn = fmaxf(fmaxf(mn, __shfl_xor(mn, 32)), m);
-                const float al = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            if (__any(mx > ref.limit)) {
+                const float top = fmaxf(mx, __shfl_xor(mx, 16)), al = ref.move(fmaxf(top, __shfl_xor(top, 32)), c);
                 l *= al;
 #pragma unroll
                 for (int i = 0; i < NB; i++) o[i] *= al;
-                m = mn;
+                shift = __any(ref.base != 0.0f);
             }
-            const float mu = m == -INFINITY ? 0.0f : m - M::kBias;
+            if (shift) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) s[r] -= ref.base;
+            }
             V4 p;
 #pragma unroll
-            for (int r = 0; r < 4; r++) { const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -mu)); l += e; p[r] = (T)e; }
+            for (int r = 0; r < 4; r++) { const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -ref.sub)); l += e; p[r] = (T)e; }
             unsigned ad[NB];
             s16x4 raw[NB];
             V4 v[NB];
@@ -431,7 +455,7 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(PagedAttn a, AttnPar
         for (int i = 0; i < NB; i++)
 #pragma unroll
             for (int r = 0; r < 4; r++) red[(wave * kStepRows + n16) * (DP + 2) + i * 16 + g4 * 4 + r] = o[i][r];
-        if (g4 == 0) { red[(wave * kStepRows + n16) * (DP + 2) + DP] = m; red[(wave * kStepRows + n16) * (DP + 2) + DP + 1] = l; }
+        if (g4 == 0) { red[(wave * kStepRows + n16) * (DP + 2) + DP] = ref.at(c); red[(wave * kStepRows + n16) * (DP + 2) + DP + 1] = l; }
         __syncthreads();
         for (int x = tid; x < (r1 - r0) * (DP / 4); x += 256) {
             const int rr = x / (DP / 4), e = (x % (DP / 4)) * 4;
@@ -577,7 +601,9 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_chunk_kernel(PagedAttn a, At
     for (int b = 0; b < NB; b++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[b][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
+    AttnRef<T> ref;
+    bool shift = false;                                                    // some row's scores are too large to do without base
+    float l = 0.0f;
     const int kf = n32 * DP * 2 + ((h ^ swz<DP>(n32)) << 4);               // K fragment ks of half kh: kb + kh * 32 rows + (kf ^ ks * 32)
     const int vrow = 4 * h + ((lane & 15) >> 2), vcol = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
     const int vf = vrow * DP * 2 + ((vcol ^ swz<DP>(vrow)) << 4) + (lane & 1) * 8;   // V^T of keys 8 x + vrow: vb + 8 x rows + (vf ^ block * 64 ^ (x & 1) * 32)
@@ -636,21 +662,25 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_chunk_kernel(PagedAttn a, At
         for (int kh = 0; kh < 2; kh++)
 #pragma unroll
             for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[kh][i]);
-        mx *= c;
-        if (__any(mx > m + M::kMove)) {
-            const float mn = fmaxf(fmaxf(mx, __shfl_xor(mx, 32)), m), al = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        if (__any(mx > ref.limit)) {
+            const float al = ref.move(fmaxf(mx, __shfl_xor(mx, 32)), c);
             l *= al;
 #pragma unroll
             for (int b = 0; b < NB; b++) o[b] *= al;
-            m = mn;
+            shift = __any(ref.base != 0.0f);
         }
-        const float mu = m == -INFINITY ? 0.0f : m - M::kBias;
+        if (shift) {
+#pragma unroll
+            for (int kh = 0; kh < 2; kh++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[kh][i] -= ref.base;
+        }
         V8 p[4];
 #pragma unroll
         for (int kh = 0; kh < 2; kh++)
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kh][i], c, -mu));
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kh][i], c, -ref.sub));
                 l += e;
                 p[kh * 2 + (i >> 3)][i & 7] = (T)e;
             }
@@ -708,7 +738,7 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_chunk_kernel(PagedAttn a, At
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int i = 0; i < 4; i++) *(f32x4 *)(ps.o + at * DP + b * 32 + 8 * i + 4 * h) = f32x4{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]};
-        if (h == 0) ps.ml[at] = make_float2(m, l);
+        if (h == 0) ps.ml[at] = make_float2(ref.at(c), l);
     }
 }
 

@@ -655,3 +655,33 @@ def test_plan_of_two_to_the_31_rows():
         for at in (0, guard + cap):
             assert L.wmi_dev_download(got.ctypes.data, a.data_ptr() + 4 * at, got.nbytes) == 0 and np.array_equal(got, mark), at
         a.free()
+
+
+# ------------------------------------------------------------------------------------------------ attention: huge scores
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (40, 4)])
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_attention_of_scores_of_any_finite_size(dtype, dim, page, new, sign):
+    """Scores up to 2^33 (float16) and 2^100 (bfloat16), positive and negative: every key is a multiple of one vector, the largest multiple
+    takes everything, and keys with the same one -- in different tiles, waves and parts -- share it evenly. (The gap to the next multiple, a
+    two-thousandth of the score, is far above the 2^-24 a score is off by.) Bound: the output's rounding and the probabilities', half a step each."""
+    rng = np.random.default_rng(dim + new)
+    n, top = 3000, 2000 if dtype == "float16" else 250
+    n_pages = -(-n // page)
+    step, hot = (16.0, 4096.0) if dtype == "float16" else (2.0 ** 40, 2.0 ** 46)
+    mult = rng.integers(top // 2, top - 1, n_pages * page) if sign > 0 else rng.integers(3, top // 2, n_pages * page)
+    best = rng.permutation(n - new)[:9]
+    mult[best] = top if sign > 0 else 2
+    k = np.broadcast_to((mult * step)[:, None, None], (n_pages * page, 1, dim))
+    v = rng.uniform(0.5, 1.5, (n_pages * page, 1, dim))
+    hosts = [host_form(x.reshape(n_pages, page, 1, dim), dtype) for x in (k, v)]
+    assert np.array_equal(values(hosts[0], dtype).reshape(-1, dim)[:, 0], mult * step)
+    q = host_form(np.broadcast_to(hot * (1 + rng.integers(0, 100, (new, 3, 1)) / 128), (new, 3, dim)), dtype)
+    cache = sv.PagedCache(*(dev(h, dtype) for h in hosts))
+    table, cu, kv = np.arange(n_pages, dtype=np.int32)[None], np.array([0, new], np.int32), np.array([n], np.int32)
+    ref = values(hosts[1], dtype).reshape(-1, dim)[best].mean(0)
+    for hint in (n, 1):                                            # keys split over workgroups, and all of them in one
+        got = values(run_attn(cache, table, q, cu, kv, dtype, new, hint, scale=sign), dtype)
+        assert np.isfinite(got).all(), hint
+        assert (np.abs(got - ref) <= 3.01 * HALF_STEP[dtype] * np.abs(ref)).all(), (hint, float(np.abs(got / ref - 1).max()))
