@@ -662,7 +662,7 @@ bool Engine::decoder_pass(std::vector<DecRow> &rows, const std::vector<SampleRow
                 const int *m = (const int *)(db + o_draw);
                 const size_t at = (sizeof(SampleOut) + sizeof(TopkOut) * 8) * (size_t)lrows_cap_;
                 int *tok = (int *)(out_dev_.as<char>() + at);
-                const DrawArgs da{logits_.p, nullptr, (const float *)m + 3 * D, (const float *)m + 4 * D, (const float *)m + D, m + 2 * D, m, tok, (float *)tok + D, (long)Vp_, D, V_, WMI_F32};
+                const DrawArgs da{logits_.p, nullptr, (const float *)m + 3 * D, (const float *)m + 4 * D, (const float *)m + D, m + 2 * D, m, tok, (float *)tok + D, (long)Vp_, D, V_, WMI_F32, d_out};
                 PROF(WMI_K_DEC_OTHER, 4.0 * D * V_, draw_tokens(da, stream_));
                 WMI_HIP_OK(hipMemcpyAsync(out_host_.as<char>() + at, tok, (sizeof(int) + sizeof(float)) * (size_t)D, hipMemcpyDeviceToHost, stream_));
             }

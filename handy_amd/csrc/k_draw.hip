@@ -573,7 +573,8 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
         a.token[row] = token;
         if (a.logprob) {
             const float v = clean((float)src[token]);
-            a.logprob[row] = (float)((v == top ? 0.0 : ((double)v - (double)top) / T64) - log((double)z * (1.0 / kMassOne)));
+            if (a.whole) a.logprob[row] = (float)((double)v / T64 - (double)a.whole[a.row_of ? a.row_of[row] : row].lse);
+            else a.logprob[row] = (float)((v == top ? 0.0 : ((double)v - (double)top) / T64) - log((double)z * (1.0 / kMassOne)));
         }
     }
 }
@@ -612,7 +613,7 @@ WHISPER_API int wmi_sample_tokens(const void *logits, int dtype, long long row_s
     if (!call.ok()) return -4;
     if (!call.own(logits, (const void *)uniform, (const void *)token) || (temperature && !call.owns(temperature)) || (top_k && !call.owns(top_k)) ||
         (top_p && !call.owns(top_p)) || (min_p && !call.owns(min_p)) || (logprob && !call.owns(logprob))) return -1;
-    const DrawArgs a{logits, temperature, top_p, min_p, uniform, top_k, nullptr, token, logprob, (long)row_stride, n_rows, n_vocab, dtype};
+    const DrawArgs a{logits, temperature, top_p, min_p, uniform, top_k, nullptr, token, logprob, (long)row_stride, n_rows, n_vocab, dtype, nullptr};
     return draw_tokens(a, st) ? 0 : -4;
 }
 

@@ -153,6 +153,7 @@ struct DrawArgs {
     float *logprob;                                               // null: not wanted
     long row_stride;
     int n_rows, n_vocab, dtype;
+    const SampleOut *whole;                                       // null, or per row of the logits: log-probabilities are relative to its lse
 };
 constexpr int kDrawMaxVocab = 262144;
 bool draw_tokens(const DrawArgs &a, hipStream_t st);

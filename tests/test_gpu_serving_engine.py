@@ -243,3 +243,35 @@ def test_device_draws_where_nothing_is_left_take_the_rows_own_token(wr, model_pa
     st.full_batch(fp, [synth_pcm(900, 45 * 16000)])
     assert prompts[0] == 2 and starts == {1: {777}, 2: {0}}, (prompts, starts)
     st.free(); ctx.free()
+
+
+def test_device_draws_have_the_hosts_log_probabilities(wr, model_path):
+    """Where the timestamps outweigh the best text token the text is masked after the row's sum was taken: the drawn timestamp's log-probability
+    is relative to that whole sum, with the device's draws as with the host's. The filter sets the rows of the first token: one text token
+    and two timestamps, whose sum is known. Bound: the sum's and the exponentials' rounding, 2^-20 of values of about 1."""
+    ctx = wr.WhisperContext(model_path("micro.en", decisive=1.0))
+    beg = ctx.token_beg()
+    x = {777: 1.0, beg + 5: 1.0, beg + 9: 0.9}
+    lse = float(np.log(np.sum(np.exp(list(x.values())))))
+
+    seen = set()
+
+    def first(tokens, logits):
+        if not tokens:
+            logits[:] = -np.inf
+            for i, v in x.items():
+                logits[i] = v
+        else:
+            seen.add((tokens[0].id, tokens[0].plog))
+    for device in (False, True):
+        seen.clear()
+        st = ctx.create_batch_state(4, 3, 4)
+        st.set_device_draws(device)
+        fp = _params(wr, 3)
+        fp.set_max_tokens(5); fp.set_filter_logits_callback(first)
+        st.full_batch(fp, [synth_pcm(910 + i, 6 * 16000) for i in range(4)])
+        assert {t for t, _ in seen} == {beg + 5, beg + 9}, (device, seen)
+        for t, p in seen:
+            assert abs(p - (x[t] - lse)) < 2.0 ** -20, (device, t, p, x[t] - lse)
+        st.free()
+    ctx.free()
