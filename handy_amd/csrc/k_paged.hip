@@ -279,10 +279,12 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(PagedAttn a, AttnPar
     const int lrow = lane / CH, lslot = lane % CH;
     const long v_minus_k = (const char *)vc - (const char *)kc;
     const T *kl[NI];                                                       // a lane's address in load i of a tile, from the tile's first key on
+    bool past[NI];                                                         // ... whose dims lie past the head's: zeros as K (q is 0 there, and infinity times 0 is none)
 #pragma unroll
     for (int i = 0; i < NI; i++) {
         const int ch = lslot ^ swz<DP>(i * RPI + lrow);
-        kl[i] = kc + (i * RPI + lrow) * a.token_stride + (ch * 8 < a.dim ? ch * 8 : 0);         // (dims past the head's: any of the key's own, q is 0 there)
+        past[i] = ch * 8 >= a.dim;
+        kl[i] = kc + (i * RPI + lrow) * a.token_stride + (past[i] ? 0 : ch * 8);                // (as V any of the key's own: what comes of them is not written)
     }
 
     for (int r0 = 0; r0 < rows; r0 += kStepRows) {
@@ -338,7 +340,7 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(PagedAttn a, AttnPar
 #pragma unroll
                 for (int i = 0; i < NI; i++) {
                     const T *k = kl[i] + off;
-                    copy(k, (const T *)((const char *)k + v_minus_k), buf, i);
+                    copy(past[i] ? (const T *)attn_zero_chunk : k, (const T *)((const char *)k + v_minus_k), buf, i);
                 }
                 return;
             }
@@ -550,8 +552,9 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_chunk_kernel(PagedAttn a, At
     // Loads: one wave instruction moves RPI keys (1 KB) of K or V; this wave's are key groups wave, wave + WV, .. of a tile. Where a
     // group lies in one page and every key of the tile exists, its address is a scalar (page, token) plus a constant of the lane;
     // the chunk a lane fetches does not depend on which of the wave's groups it is.
-    const int lrow = lane / CH, lslot = lane % CH, lch = lslot ^ swz<DP>(wave * RPI + lrow), dch = lch * 8 < a.dim ? lch * 8 : 0;
-    const T *kl = kc + lrow * a.token_stride + dch;                        // (dims past the head's: any of the key's own, q is 0 there)
+    const int lrow = lane / CH, lslot = lane % CH, lch = lslot ^ swz<DP>(wave * RPI + lrow);
+    const bool past = lch * 8 >= a.dim;                                    // dims past the head's: zeros as K (q is 0 there, and infinity times 0 is none)
+    const T *kl = kc + lrow * a.token_stride + (past ? 0 : lch * 8);       // (as V any of the key's own: what comes of them is not written)
     const long v_minus_k = (const char *)vc - (const char *)kc;
     int pages;                                                             // lane l: page of key group l of the tile that is loaded next
     auto entries = [&](int t) { const int j = t * kChunkKeys + (lane & (kChunkKeys / RPI - 1)) * RPI; return tbl[min(max(j, lo), hi - 1) >> a.lp]; };
@@ -573,7 +576,7 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_chunk_kernel(PagedAttn a, At
             for (int i = 0; i < NI; i++) {
                 const int page = __builtin_amdgcn_readlane(pages, wave + WV * i), token = (k0 + (wave + WV * i) * RPI) & ((1 << a.lp) - 1);
                 const T *k = kl + (page * a.page_stride + token * a.token_stride);
-                copy(k, (const T *)((const char *)k + v_minus_k), buf, i);
+                copy(past ? (const T *)attn_zero_chunk : k, (const T *)((const char *)k + v_minus_k), buf, i);
             }
         } else {                                                           // a tile at an end of the keys, or with a page that is not there
             bool bad = false;

@@ -685,3 +685,30 @@ def test_attention_of_scores_of_any_finite_size(dtype, dim, page, new, sign):
         got = values(run_attn(cache, table, q, cu, kv, dtype, new, hint, scale=sign), dtype)
         assert np.isfinite(got).all(), hint
         assert (np.abs(got - ref) <= 3.01 * HALF_STEP[dtype] * np.abs(ref)).all(), (hint, float(np.abs(got / ref - 1).max()))
+
+
+# ------------------------------------------------------------------------------------------------ attention: infinite keys
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim,page", [(40, 16), (64, 16), (80, 64), (128, 32), (72, 2)])
+@pytest.mark.parametrize("new", [1, 50])
+def test_attention_of_keys_at_minus_infinity(dtype, dim, page, new):
+    """Keys with an infinite element (in the first dims, in the last) that make the score minus infinity have weight 0, whatever the head's dim:
+    the result is the other keys'."""
+    rng = np.random.default_rng(dim + new)
+    n = 700
+    n_pages = -(-n // page)
+    k, v = (rng.standard_normal((n_pages * page, 2, dim)) for _ in range(2))
+    q = rng.standard_normal((new, 4, dim))
+    q[:, :, 0], q[:, :, -1] = np.abs(q[:, :, 0]) + 0.1, np.abs(q[:, :, -1]) + 0.1
+    gone = rng.random(n_pages * page) < 0.3
+    gone[0] = False
+    keep = [host_form(x.reshape(n_pages, page, 2, dim), dtype) for x in (k, v)]
+    k[gone & (np.arange(len(gone)) % 2 == 0), :, 0] = -np.inf
+    k[gone & (np.arange(len(gone)) % 2 == 1), :, -1] = -np.inf
+    cache = sv.PagedCache(dev(host_form(k.reshape(n_pages, page, 2, dim), dtype), dtype), dev(keep[1], dtype))
+    table, cu, kv = np.arange(n_pages, dtype=np.int32)[None], np.array([0, new], np.int32), np.array([n], np.int32)
+    q = host_form(q, dtype)
+    got = run_attn(cache, table, q, cu, kv, dtype, new, n)
+    # the restatement over one page a key, the gone ones' page absent
+    one = [h.reshape(n_pages * page, 1, 2, dim) for h in keep]
+    check_attn(got, dtype, q, one, np.where(gone, -1, np.arange(n_pages * page))[None], cu, kv, 1, dim ** -0.5, what=(dim, new))
