@@ -212,11 +212,13 @@ __device__ __forceinline__ AttnReq attn_req(const PagedAttn &a, int cu0, int cu1
     return r;
 }
 __device__ __forceinline__ AttnReq attn_req(const PagedAttn &a, int i) { return attn_req(a, a.cu[i], a.cu[i + 1], a.kv_lens[i]); }
+// the first key that the row at position `pos` sees (a position in front of the keys and a window of 2^31 - 1 do not overflow)
+__device__ __forceinline__ int attn_first_key(const PagedAttn &a, int pos) { return a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0; }
 // keys [lo, hi) that the packed rows r0 .. r1 - 1 of a request see between them
 __device__ __forceinline__ void attn_keys(const PagedAttn &a, const AttnReq &q, int r0, int r1, int &lo, int &hi) {
     const int first = q.len - q.n + r0 / a.group, last = q.len - q.n + (r1 - 1) / a.group;
     hi = max(last + 1, 0);
-    lo = a.window > 0 ? max(first - a.window + 1, 0) : 0;
+    lo = attn_first_key(a, first);
 }
 // how many parts the keys of a tile of rows are cut into: at most `splits`, none shorter than `least` key tiles
 __device__ __forceinline__ int attn_parts(int n_kt, int splits, int least) { return max(1, min(splits, n_kt / least)); }
@@ -295,7 +297,7 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(PagedAttn a, AttnPar
         if (part >= parts) continue;
         const int t0 = kt0 + (int)((long)n_kt * part / parts) + wave, t1 = kt0 + (int)((long)n_kt * (part + 1) / parts);
         const int row = min(r0 + n16, r1 - 1), tok = row / a.group, hq = head * a.group + row % a.group, pos = rq.len - rq.n + tok;
-        const int first = rq.len - rq.n + r0 / a.group, klow = a.window > 0 ? pos - a.window + 1 : 0;
+        const int first = rq.len - rq.n + r0 / a.group, klow = attn_first_key(a, pos);
         const bool one = r0 / a.group == (r1 - 1) / a.group;               // one token: every key in [lo, hi) is seen by every row
         V8 qf[NK];
 #pragma unroll
@@ -539,7 +541,8 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_chunk_kernel(PagedAttn a, At
     const int w0 = r0 + wave * 32, row = min(w0 + n32, r1 - 1), tok = row / a.group, hq = head * a.group + row % a.group, pos = rq.len - rq.n + tok;
     const bool busy = w0 < r1;
     const int pmin = rq.len - rq.n + w0 / a.group, pmax = rq.len - rq.n + (min(w0 + 32, r1) - 1) / a.group;   // this wave's positions
-    const int klow = a.window > 0 ? pos - a.window + 1 : 0;
+    const int klow_min = attn_first_key(a, pmin), klow_max = attn_first_key(a, pmax);
+    const int klow = attn_first_key(a, pos);
     V8 qf[NK];
 #pragma unroll
     for (int ks = 0; ks < NK; ks++) {
@@ -627,7 +630,7 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_chunk_kernel(PagedAttn a, At
         const int buf = (t - t0) & 1, k0 = t * kChunkKeys;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // everybody's share of this tile has landed, the other buffer is free
         if (t + 1 < t1) { stage(t + 1, buf ^ 1); pages = entries(t + 2); }
-        if (!busy || k0 > pmax || (a.window > 0 && k0 + kChunkKeys <= pmin - a.window + 1)) continue;
+        if (!busy || k0 > pmax || k0 + kChunkKeys <= klow_min) continue;
         const char *kb = smem + buf * 2 * TILE, *vb = kb + TILE;
         f32x16 s[2];
 #pragma unroll
@@ -641,7 +644,7 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_chunk_kernel(PagedAttn a, At
 #pragma unroll
         for (int w = 0; w < WV; w++) flags |= bad_flag[buf][w];
         const bool hole = __builtin_amdgcn_readfirstlane(flags) != 0;
-        const bool mixed = k0 + kChunkKeys - 1 > pmin || (a.window > 0 && k0 < pmax - a.window + 1) || hole;
+        const bool mixed = k0 + kChunkKeys - 1 > pmin || k0 < klow_max || hole;
         if (mixed) {
 #pragma unroll
             for (int kh = 0; kh < 2; kh++)

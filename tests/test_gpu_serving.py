@@ -712,3 +712,14 @@ def test_attention_of_keys_at_minus_infinity(dtype, dim, page, new):
     # the restatement over one page a key, the gone ones' page absent
     one = [h.reshape(n_pages * page, 1, 2, dim) for h in keep]
     check_attn(got, dtype, q, one, np.where(gone, -1, np.arange(n_pages * page))[None], cu, kv, 1, dim ** -0.5, what=(dim, new))
+
+
+@pytest.mark.parametrize("news", [[4, 1, 9], [90, 7, 300]])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 5, 40, 2, 1])
+def test_attention_windows_as_long_as_they_come_and_more_rows_than_keys(news, window):
+    """A window of 2^31 - 1 as "no limit", with requests that bring more new tokens than they have keys: their first rows, at positions in front
+    of the keys, give zeros, the others see what they see."""
+    lens = [2, 0, 5] if max(news) < 10 else [60, 3, 250]
+    cache, hosts, _, table, q, cu, kv = attn_setup(7, "bfloat16", lens, news, 2, 3, 64, 16)
+    got = run_attn(cache, table, q, cu, kv, "bfloat16", max(news), max(lens), window=window, extra_rows=2)
+    check_attn(got, "bfloat16", q, hosts, table, cu, kv, 16, 64 ** -0.5, window, (news, window))
