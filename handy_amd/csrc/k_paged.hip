@@ -865,6 +865,7 @@ int fill_attn(const wmi_paged_cache *c, const wmi_paged_attn *p, PagedAttn &a) {
     if (!(p->scale == p->scale) || p->scale - p->scale != 0.0f) return -1;          // NaN or infinite
     if (c->head_dim % 8 || c->head_dim > 128 || p->n_q_heads / c->n_kv_heads > 128) return -3;
     if ((long long)p->n_rows * p->n_q_heads > 0x3fffffffLL || (long long)p->n_seq * c->n_kv_heads > 0x3fffffLL) return -3;      // workgroup and packed row numbers are 32-bit
+    if ((long long)p->table_cols * c->page_tokens > 0x7fffff00LL) return -3;      // key numbers are 32-bit, and the kernels' run up to 255 past the last
     a.k = c->k; a.v = c->v; a.dtype = c->dtype; a.n_pages = c->n_pages; a.lp = log2_of(c->page_tokens); a.hkv = c->n_kv_heads; a.dim = c->head_dim;
     a.page_stride = c->page_stride; a.token_stride = c->token_stride; a.head_stride = c->head_stride;
     a.group = p->n_q_heads / c->n_kv_heads; a.n_rows = p->n_rows; a.n_seq = p->n_seq; a.cols = p->table_cols; a.table_stride = p->table_stride;

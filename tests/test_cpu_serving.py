@@ -186,3 +186,12 @@ def test_tables_whose_rows_share_memory_are_refused():
         assert sv._table(Fake((1, 8), "int32", (stride, 1)), 1) == (0x10000, 8, 8)
     assert sv._table(Fake((3, 8), "int32", (11, 1)), 3) == (0x10000, 11, 8)
     assert sv._table(Fake((3, 0), "int32", (0, 1)), 3)[1:] == (0, 0)
+
+
+def test_attention_refuses_tables_of_more_keys_than_its_numbers_hold():
+    """Key numbers are 32-bit and run a few tiles past the last one: table_cols * page_tokens is at most 2^31 - 256, in the workspace call too."""
+    L = wr.load_library()
+    for page, cols, rc in ((16, 2 ** 27 - 16, -1), (16, 2 ** 27 - 15, -3), (16, 2 ** 31 - 1, -3), (1, 2 ** 31 - 256, -1), (1, 2 ** 31 - 255, -3), (1024, 2 ** 21 - 1, -1), (1024, 2 ** 21, -3)):
+        c, a = cache_struct(page_tokens=page), attn_struct(table_cols=cols, table_stride=cols)
+        assert L.wmi_paged_attention(C.byref(c), C.byref(a), None, 0, None) in ((rc, -4) if rc == -1 else (rc,)), (page, cols)      # (-1: no device memory; -4: no GPU at all)
+        assert (L.wmi_paged_attention_workspace(C.byref(c), C.byref(a)) >= 0) == (rc == -1)
