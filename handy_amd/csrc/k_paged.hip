@@ -847,9 +847,9 @@ namespace {
 int log2_of(int x) { int l = 0; while ((1 << l) < x) l++; return l; }
 bool power_of_two(int x) { return x > 0 && !(x & (x - 1)); }
 
-// what every entry asks of a cache description; 0, -1 or -3
+// what every entry asks of a cache description, its memory apart; 0, -1 or -3
 int check_cache(const wmi_paged_cache *c) {
-    if (!c || !c->k || !c->v || c->n_pages < 1 || c->n_kv_heads < 1 || c->head_dim < 1) return -1;
+    if (!c || c->n_pages < 1 || c->n_kv_heads < 1 || c->head_dim < 1) return -1;
     if (c->dtype != WMI_F16 && c->dtype != WMI_BF16) return -1;
     if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0) return -1;
     if (!power_of_two(c->page_tokens) || c->page_tokens > 1024 || (long long)c->n_pages * c->page_tokens > 0x7fffffffLL) return -3;
@@ -914,7 +914,7 @@ WHISPER_API int wmi_paged_write(const wmi_paged_cache *cache, const void *k_new,
                                 long long v_row_stride, long long v_head_stride, const int *slots, int n_rows, void *stream) {
     const int rc = check_cache(cache);
     if (rc) return rc;
-    if (n_rows < 0 || (n_rows > 0 && (!k_new || !v_new || !slots)) || k_row_stride < 0 || k_head_stride < 0 || v_row_stride < 0 || v_head_stride < 0) return -1;
+    if (!cache->k || !cache->v || n_rows < 0 || (n_rows > 0 && (!k_new || !v_new || !slots)) || k_row_stride < 0 || k_head_stride < 0 || v_row_stride < 0 || v_head_stride < 0) return -1;
     if (n_rows == 0) return 0;
     if (cache->k == cache->v && (k_new != v_new || k_row_stride != v_row_stride || k_head_stride != v_head_stride)) return -1;      // two values for one place
     hipStream_t st = (hipStream_t)stream;
@@ -946,6 +946,7 @@ WHISPER_API int wmi_paged_attention(const wmi_paged_cache *cache, const wmi_page
     PagedAttn a;
     const int rc = fill_attn(cache, args, a);
     if (rc) return rc;
+    if (!a.k || !a.v) return -1;
     if (a.n_rows == 0 || a.n_seq == 0) return 0;
     if (!a.q || !a.out || !a.cu || !a.kv_lens || (a.cols > 0 && !a.table) || a.table_stride < a.cols) return -1;
     const long long all = a.page_stride | a.token_stride | a.head_stride | a.q_row | a.q_head | a.o_row | a.o_head;

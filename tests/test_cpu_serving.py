@@ -195,3 +195,15 @@ def test_attention_refuses_tables_of_more_keys_than_its_numbers_hold():
         c, a = cache_struct(page_tokens=page), attn_struct(table_cols=cols, table_stride=cols)
         assert L.wmi_paged_attention(C.byref(c), C.byref(a), None, 0, None) in ((rc, -4) if rc == -1 else (rc,)), (page, cols)      # (-1: no device memory; -4: no GPU at all)
         assert (L.wmi_paged_attention_workspace(C.byref(c), C.byref(a)) >= 0) == (rc == -1)
+
+
+def test_workspace_sizes_need_no_cache_memory():
+    """The workspace call looks at sizes only: a caller may size its memory before it allocates the cache. The calls that use the cache refuse."""
+    L = wr.load_library()
+    a = attn_struct(q=None, out=None, block_table=None, cu_q=None, kv_lens=None, n_rows=1, n_seq=1, max_kv=100000, table_cols=8000, table_stride=8000)
+    need = L.wmi_paged_attention_workspace(C.byref(cache_struct()), C.byref(a))
+    assert need > 0
+    for kw in (dict(k=None), dict(v=None), dict(k=None, v=None)):
+        assert L.wmi_paged_attention_workspace(C.byref(cache_struct(**kw)), C.byref(a)) == need
+        assert L.wmi_paged_attention(C.byref(cache_struct(**kw)), C.byref(attn_struct()), None, 0, None) == -1
+        assert L.wmi_paged_write(C.byref(cache_struct(**kw)), P, 128, 64, P, 128, 64, P, 3, None) == -1
