@@ -60,7 +60,7 @@ class DeviceArray:
         """Another shape over the same memory; strides and offset in elements."""
         root = self._base or self
         last = self._offset + offset + sum((s - 1) * t for s, t in zip(shape, strides))
-        if min(strides, default=0) < 0 or (0 not in shape and last >= math.prod(root.shape)):
+        if min(strides, default=0) < 0 or self._offset + offset < 0 or (0 not in shape and last >= math.prod(root.shape)):
             raise ValueError("view outside the array")
         return DeviceArray(shape, self.dtype, root, strides, self._offset + offset)
 

@@ -207,3 +207,19 @@ def test_workspace_sizes_need_no_cache_memory():
         assert L.wmi_paged_attention_workspace(C.byref(cache_struct(**kw)), C.byref(a)) == need
         assert L.wmi_paged_attention(C.byref(cache_struct(**kw)), C.byref(attn_struct()), None, 0, None) == -1
         assert L.wmi_paged_write(C.byref(cache_struct(**kw)), P, 128, 64, P, 128, 64, P, 3, None) == -1
+
+
+def test_views_stay_inside_their_array():
+    """DeviceArray.view: neither end may lie outside the memory, for views of views too."""
+    base = sv.DeviceArray((1,), "int32", _base=Fake((100,), "int32"))          # (stands for an allocation: the checks look at shapes only)
+    base._base, base.shape, base._strides = None, (100,), (1,)
+    for shape, strides, offset in (((4,), (1,), -1), ((4,), (1,), -100), ((4,), (1,), 97), ((1,), (1,), 100), ((2, 3), (50, 26), 0), ((2,), (-1,), 5)):
+        with pytest.raises(ValueError):
+            base.view(shape, strides, offset)
+    inner = base.view((10,), (1,), 20)
+    assert inner._offset == 20 and inner.view((5,), (1,), -20)._offset == 0    # a view's offset counts from the view, the memory is the array's
+    with pytest.raises(ValueError):
+        inner.view((5,), (1,), -21)
+    with pytest.raises(ValueError):
+        base.view((0, 4), (4, 1), -8)
+    assert base.view((0, 4), (4, 1), 100).shape == (0, 4)
