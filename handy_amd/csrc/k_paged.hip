@@ -857,6 +857,35 @@ int check_cache(const wmi_paged_cache *c) {
 }
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
+// whether two [rows][heads][dim] arrays of the same strides share an element, the second `delta` elements behind the first (self: an
+// array with itself, two of its rows or heads)
+bool rows_meet(long delta, long rows, long heads, long dim, long row, long head, bool self) {
+    if (self && ((head >= dim && row >= head * (heads - 1) + dim) || (row >= dim && head >= row * (rows - 1) + dim))) return false;      // one axis inside the other
+    for (long dh = 1 - heads; dh < heads; dh++) {
+        const long x = delta - dh * head, d0 = row > 0 ? x / row : 0;
+        for (long d = d0 - 1; d <= d0 + 1; d++) {                       // the nearest row steps there are
+            const long dr = d < 1 - rows ? 1 - rows : d > rows - 1 ? rows - 1 : d, gap = x - dr * row;
+            if (gap > -dim && gap < dim && !(self && dh == 0 && dr == 0)) return true;
+        }
+    }
+    return false;
+}
+// whether what attention writes (out, the workspace) meets anything else of the call
+bool attn_shares(const PagedAttn &a, const void *workspace, size_t ws_bytes) {
+    struct Span { uintptr_t at, end; };
+    auto span = [](const void *p, long bytes) { return Span{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes}; };
+    auto meet = [](Span x, Span y) { return x.at < y.end && y.at < x.end; };
+    const long heads = (long)a.hkv * a.group, kv = 2 * ((a.n_pages - 1) * a.page_stride + ((1L << a.lp) - 1) * a.token_stride + (a.hkv - 1) * a.head_stride + a.dim);
+    const Span q = span(a.q, 2 * ((a.n_rows - 1) * a.q_row + (heads - 1) * a.q_head + a.dim)), out = span(a.out, 2 * ((a.n_rows - 1) * a.o_row + (heads - 1) * a.o_head + a.dim));
+    const Span ws = span(workspace, (long)ws_bytes);
+    const Span other[] = {span(a.k, kv), span(a.v, kv), span(a.table, a.cols > 0 ? 4 * ((a.n_seq - 1) * a.table_stride + a.cols) : 0), span(a.cu, 4 * (a.n_seq + 1L)), span(a.kv_lens, 4L * a.n_seq)};
+    for (const Span &o : other) if (meet(out, o) || (ws_bytes > 0 && meet(ws, o))) return true;
+    if (ws_bytes > 0 && (meet(ws, q) || meet(ws, out))) return true;
+    if (rows_meet(0, a.n_rows, heads, a.dim, a.o_row, a.o_head, true)) return true;
+    // q and out may be parts of one buffer's rows: spans that meet are looked at closely if their strides are alike
+    return meet(out, q) && (a.q_row != a.o_row || a.q_head != a.o_head || rows_meet(((long)out.at - (long)q.at) / 2, a.n_rows, heads, a.dim, a.o_row, a.o_head, false));
+}
+
 // the description in the kernels' terms, checked; 0, -1 or -3
 int fill_attn(const wmi_paged_cache *c, const wmi_paged_attn *p, PagedAttn &a) {
     const int rc = check_cache(c);
@@ -951,13 +980,15 @@ WHISPER_API int wmi_paged_attention(const wmi_paged_cache *cache, const wmi_page
     if (!a.q || !a.out || !a.cu || !a.kv_lens || (a.cols > 0 && !a.table) || a.table_stride < a.cols) return -1;
     const long long all = a.page_stride | a.token_stride | a.head_stride | a.q_row | a.q_head | a.o_row | a.o_head;
     if (all % 8 || a.q_row < 0 || a.q_head < 0 || a.o_row < 0 || a.o_head < 0 || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.q) || !aligned16(a.out)) return -1;
+    const size_t need = paged_attention_workspace(a);
+    if (need > workspace_bytes) return -2;
+    if (need > 0 && (!workspace || !aligned16(workspace))) return -1;
+    if (attn_shares(a, workspace, need)) return -1;
     hipStream_t st = (hipStream_t)stream;
     const ServeCall call(st);
     if (!call.ok()) return -4;
     if (!call.own(a.k, a.v, a.q, (const void *)a.out, (const void *)a.cu, (const void *)a.kv_lens) || (a.cols > 0 && !call.owns(a.table))) return -1;
-    const size_t need = paged_attention_workspace(a);
-    if (need > workspace_bytes) return -2;
-    if (need > 0 && (!aligned16(workspace) || !call.owns(workspace))) return -1;
+    if (need > 0 && !call.owns(workspace)) return -1;
     return paged_attention(a, workspace, st) ? 0 : -4;
 }
 

@@ -137,7 +137,7 @@ def _lib():
 
 def _check(rc: int, what: str):
     if rc in (-1, -2, -3):
-        raise ValueError(what + {-1: ": bad arguments (sizes, alignment, or memory that is not the call's GPU's)", -2: ": workspace too small",
+        raise ValueError(what + {-1: ": bad arguments (sizes, alignment, outputs that share memory, or memory that is not the call's GPU's)", -2: ": workspace too small",
                                  -3: ": sizes not supported"}[rc])
     if rc != 0:
         raise wr.WhisperError(f"{what} failed", rc)

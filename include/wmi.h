@@ -301,8 +301,9 @@ WHISPER_API int wmi_paged_write(const wmi_paged_cache *cache, const void *k_new,
  * kv_lens[i] tokens: row t of n stands at position kv_lens[i] - n + t and sees the keys up to its own position, with window > 0
  * only the last `window` of them. Query heads share key heads in runs of n_q_heads / n_kv_heads (<= 128). Keys on pages that the
  * cache does not have (table entry negative or >= n_pages) are left out; a row that sees no key gives zeros; rows past
- * cu_q[n_seq] are left as they are. out shares no memory with what is read. head_dim a multiple of 8 up to 128; 16-byte aligned pointers, strides
- * multiples of 8; table_cols * page_tokens at most 2^31 - 256.
+ * cu_q[n_seq] are left as they are. out and the workspace share no memory with what is read, nor out's rows with each other (-1;
+ * q and out of the same strides may interleave in one buffer). head_dim a multiple of 8 up to 128; 16-byte aligned pointers,
+ * strides multiples of 8; table_cols * page_tokens at most 2^31 - 256.
  * max_new and max_kv: the longest request's new and total tokens, as far as the caller knows (they steer how the work is split,
  * larger or smaller values change no result beyond rounding; 0: not known). Scores, softmax and sums are 32-bit; the
  * probabilities are rounded to the cache's type for the product with V (F16: those under 2^-25 of a row's largest keep fewer than 11

@@ -223,3 +223,44 @@ def test_views_stay_inside_their_array():
     with pytest.raises(ValueError):
         base.view((0, 4), (4, 1), -8)
     assert base.view((0, 4), (4, 1), 100).shape == (0, 4)
+
+
+def test_attention_refuses_an_output_that_shares_memory():
+    """out (and the workspace) may share no element with what the kernels read, nor out's rows with each other. Layouts that interleave without
+    meeting are taken. Told from the codes without a GPU: -1 for the arguments, -4 for a call whose arguments are in order."""
+    L = wr.load_library()
+    A, far = 0x100000, dict(q=0x1000000, out=0x2000000, block_table=0x3000000, cu_q=0x3100000, kv_lens=0x3200000)
+    cache = cache_struct(k=0x4000000, v=0x5000000)
+    base = dict(far, n_rows=6, n_seq=3, n_q_heads=4, q_row_stride=256, q_head_stride=64, out_row_stride=256, out_head_stride=64, max_new=2)
+
+    def call(ws=None, ws_bytes=0, **kw):
+        return L.wmi_paged_attention(C.byref(cache), C.byref(attn_struct(**{**base, **kw})), ws, ws_bytes, None)
+    if call() != -4:
+        pytest.skip("a GPU is present: these addresses are refused as no memory of it")
+
+    def refused(**kw):
+        rc = call(**kw)
+        assert rc in (-1, -4), rc
+        return rc == -1
+    for other, size in (("q", 6 * 256 * 2), ("block_table", 3 * 8 * 4), ("cu_q", 16), ("kv_lens", 12)):
+        at, end = base[other], base[other] + size
+        for out in (at, (end - 1) // 16 * 16, at - (5 * 256 + 3 * 64 + 64) * 2 + 16):
+            assert refused(out=out), (other, hex(out))
+        assert not refused(out=(end + 15) // 16 * 16) and not refused(out=at - 6 * 256 * 2), other
+    for at in (cache.k, cache.v):
+        assert refused(out=at) and refused(out=at + 8 * 2048 * 2 - 16) and not refused(out=at + 8 * 2048 * 2)
+    both = dict(q_row_stride=1024, out_row_stride=1024)           # parts of one buffer's rows
+    assert not refused(q=A, out=A + 512, **both) and not refused(q=A + 512, out=A, **both) and refused(q=A, out=A + 496, **both) and refused(q=A, out=A, **both)
+    heads = dict(q_row_stride=512, out_row_stride=512, q_head_stride=128, out_head_stride=128)      # every other head of one buffer
+    assert not refused(q=A, out=A + 128, **heads) and refused(q=A, out=A + 112, **heads) and refused(q=A, out=A + 256, **heads) and refused(q=A, out=A + 1024, **heads)
+    for kw in (dict(out_row_stride=0), dict(out_head_stride=0), dict(out_head_stride=56), dict(out_row_stride=248), dict(out_row_stride=64)):
+        assert refused(**kw), kw
+    assert not refused(out_row_stride=64, out_head_stride=6 * 64)                                  # heads outermost
+    assert not refused(n_rows=1, out_row_stride=0) and refused(n_rows=2, out_row_stride=0)
+    assert not refused(q_row_stride=0) and not refused(q_head_stride=0)                            # queries may share memory: they are read
+    long = dict(n_rows=3, n_seq=3, max_new=1, max_kv=100000, table_cols=8000, table_stride=8000)
+    need = L.wmi_paged_attention_workspace(C.byref(cache), C.byref(attn_struct(**{**base, **long})))
+    assert need > 0
+    for name in ("q", "out", "block_table", "cu_q", "kv_lens"):
+        assert refused(ws=base[name], ws_bytes=need, **long) and refused(ws=base[name] // 16 * 16 - (need - 1) // 16 * 16, ws_bytes=need, **long), name
+    assert refused(ws=cache.k, ws_bytes=need, **long) and refused(ws=cache.v, ws_bytes=need, **long) and not refused(ws=0x6000000, ws_bytes=need, **long)
