@@ -579,21 +579,19 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
     }
 }
 
-template <class T> static void draw_launch(const DrawArgs &a, hipStream_t st) {
+template <class T> static bool draw_launch(const DrawArgs &a, hipStream_t st) {
     // Short rows: four waves a row, so that more rows share a compute unit. Else sixteen if every row has a compute unit of its own
     // (256), or eight, two rows a compute unit, whose waits then fall under the other's arithmetic (1024 rows of 51866 entries: 99 us
     // against 125). Longer rows take sixteen again: a thread's share is long enough (600 rows of 262144: 317 us against 360).
-    if (a.n_vocab <= 16384) hipLaunchKernelGGL((draw_kernel<T, 256>), dim3(a.n_rows), dim3(256), 0, st, a);
-    else if (a.n_rows > 256 && a.n_vocab <= 131072) hipLaunchKernelGGL((draw_kernel<T, 512>), dim3(a.n_rows), dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((draw_kernel<T, 1024>), dim3(a.n_rows), dim3(1024), 0, st, a);
+    if (a.n_vocab <= 16384) return serve_launch(draw_kernel<T, 256>, dim3(a.n_rows), dim3(256), 0, st, a);
+    if (a.n_rows > 256 && a.n_vocab <= 131072) return serve_launch(draw_kernel<T, 512>, dim3(a.n_rows), dim3(512), 0, st, a);
+    return serve_launch(draw_kernel<T, 1024>, dim3(a.n_rows), dim3(1024), 0, st, a);
 }
 
 bool draw_tokens(const DrawArgs &a, hipStream_t st) {
     if (a.n_rows <= 0) return true;
-    if (a.dtype == WMI_F32) draw_launch<float>(a, st);
-    else if (a.dtype == WMI_F16) draw_launch<f16>(a, st);
-    else draw_launch<__bf16>(a, st);
-    return hipGetLastError() == hipSuccess;
+    if (a.dtype == WMI_F32) return draw_launch<float>(a, st);
+    return a.dtype == WMI_F16 ? draw_launch<f16>(a, st) : draw_launch<__bf16>(a, st);
 }
 
 }  // namespace wmi

@@ -821,20 +821,18 @@ template <class T, int DP> static bool attn_launch(const PagedAttn &a, void *wor
     const AttnShape s = attn_shape(a);
     const long pairs = (long)a.n_rows * a.hkv * a.group;
     const AttnParts ps{(float *)workspace, (float2 *)((float *)workspace + (s.splits == 1 ? 0 : s.splits * pairs * DP)), s.splits};
-    const unsigned join = (unsigned)pairs;
+    const dim3 join((unsigned)pairs);
+    bool ok;
     if (s.step) {
         const dim3 grid((unsigned)(a.n_seq * a.hkv), s.splits);
-        if (a.lp >= 4) hipLaunchKernelGGL((paged_step_kernel<T, DP, true>), grid, dim3(256), 0, st, a, ps);
-        else hipLaunchKernelGGL((paged_step_kernel<T, DP, false>), grid, dim3(256), 0, st, a, ps);
-        if (s.splits > 1) hipLaunchKernelGGL((paged_join_kernel<T, DP, kStepRows, kStepKeys, kStepLeast>), dim3(join), dim3(256), 0, st, a, ps);
+        ok = serve_launch(a.lp >= 4 ? paged_step_kernel<T, DP, true> : paged_step_kernel<T, DP, false>, grid, dim3(256), 0, st, a, ps);
+        if (s.splits > 1) ok = ok && serve_launch(paged_join_kernel<T, DP, kStepRows, kStepKeys, kStepLeast>, join, dim3(256), 0, st, a, ps);
     } else {
         const dim3 grid((unsigned)((long)s.tiles * a.hkv * s.splits)), threads(64 * s.waves);
-        if (s.waves == 8) hipLaunchKernelGGL((paged_chunk_kernel<T, DP, 8>), grid, threads, 0, st, a, ps, s.tiles);
-        else hipLaunchKernelGGL((paged_chunk_kernel<T, DP, 4>), grid, threads, 0, st, a, ps, s.tiles);
-        if (s.splits > 1 && s.waves == 8) hipLaunchKernelGGL((paged_join_kernel<T, DP, 256, kChunkKeys, kChunkLeast>), dim3(join), dim3(256), 0, st, a, ps);
-        else if (s.splits > 1) hipLaunchKernelGGL((paged_join_kernel<T, DP, 128, kChunkKeys, kChunkLeast>), dim3(join), dim3(256), 0, st, a, ps);
+        ok = serve_launch(s.waves == 8 ? paged_chunk_kernel<T, DP, 8> : paged_chunk_kernel<T, DP, 4>, grid, threads, 0, st, a, ps, s.tiles);
+        if (s.splits > 1) ok = ok && serve_launch(s.waves == 8 ? paged_join_kernel<T, DP, 256, kChunkKeys, kChunkLeast> : paged_join_kernel<T, DP, 128, kChunkKeys, kChunkLeast>, join, dim3(256), 0, st, a, ps);
     }
-    return hipGetLastError() == hipSuccess;
+    return ok;
 }
 
 bool paged_attention(const PagedAttn &a, void *workspace, hipStream_t st) {
@@ -935,8 +933,7 @@ WHISPER_API int wmi_paged_plan(const int *ctx_lens, const int *new_lens, int n_s
     // rows beyond two a thread are spread over workgroups, one a CU at most, each of which repeats the prefix sum (4096 requests and 303 000
     // rows, the whole call: 11.8 us with 2048 rows a workgroup, 12.0 with 1024, 14.0 with 4096)
     const int want = n_rows_cap / 2048 + (n_rows_cap % 2048 != 0), groups = want < 1 ? 1 : want > 256 ? 256 : want;
-    hipLaunchKernelGGL(paged_plan_kernel, dim3(groups), dim3(kPlanThreads), lds, st, a);
-    return serve_done();
+    return serve_launch(paged_plan_kernel, dim3(groups), dim3(kPlanThreads), lds, st, a) ? 0 : -4;
 }
 
 WHISPER_API int wmi_paged_write(const wmi_paged_cache *cache, const void *k_new, long long k_row_stride, long long k_head_stride, const void *v_new,
@@ -960,9 +957,7 @@ WHISPER_API int wmi_paged_write(const wmi_paged_cache *cache, const void *k_new,
                 (long)cache->n_pages * cache->page_tokens, (long)n_rows * cache->n_kv_heads * chunks, log2_of(cache->page_tokens), cache->n_kv_heads, chunks};
     const long want = (a.total + 255) / 256;
     const unsigned blocks = (unsigned)(want > 65536 ? 65536 : want);
-    if (wide) hipLaunchKernelGGL(paged_write_kernel<f32x4>, dim3(blocks), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(paged_write_kernel<unsigned short>, dim3(blocks), dim3(256), 0, st, a);
-    return serve_done();
+    return serve_launch(wide ? paged_write_kernel<f32x4> : paged_write_kernel<unsigned short>, dim3(blocks), dim3(256), 0, st, a) ? 0 : -4;
 }
 
 WHISPER_API long long wmi_paged_attention_workspace(const wmi_paged_cache *cache, const wmi_paged_attn *args) {

@@ -30,6 +30,12 @@ private:
     int dev_ = -1, prev_ = -1;
 };
 
-inline int serve_done() { return hipGetLastError() == hipSuccess ? 0 : -4; }
+// A launch by its own status: the runtime's last error may be another call's, from before, and is neither reported nor cleared.
+template <class... P> inline bool serve_launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t st, P... args) {
+    void *ptrs[] = {(void *)&args...};
+    if (hipLaunchKernel((const void *)kernel, grid, block, ptrs, lds, st) == hipSuccess) return true;
+    (void)hipGetLastError();
+    return false;
+}
 
 }  // namespace wmi

@@ -260,7 +260,8 @@ WHISPER_API int wmi_node_run_custom(int n_workers, int n_utts, int batch, wmi_no
  * `stream` (a hipStream_t) belongs to, or with NULL (the null stream) the calling thread's current one; host memory or another
  * GPU's is refused. Everything is enqueued on `stream`; nothing waits, allocates or keeps state, so calls may be captured into
  * graphs and made from several threads. Strides count elements. 0 ok, -1 bad arguments, -2 workspace too small, -3 sizes not
- * supported, -4 HIP error; a call that is refused does nothing. */
+ * supported, -4 HIP error (of this call; one that another call left with the runtime stays there); a call that is refused does
+ * nothing. */
 enum wmi_dtype { WMI_F16 = 0, WMI_BF16 = 1, WMI_F32 = 2 };
 
 /* K and V of one layer: element e of token t of page p, head h at k + p * page_stride + t * token_stride + h * head_stride + e,

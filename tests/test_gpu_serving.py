@@ -723,3 +723,28 @@ def test_attention_windows_as_long_as_they_come_and_more_rows_than_keys(news, wi
     cache, hosts, _, table, q, cu, kv = attn_setup(7, "bfloat16", lens, news, 2, 3, 64, 16)
     got = run_attn(cache, table, q, cu, kv, "bfloat16", max(news), max(lens), window=window, extra_rows=2)
     check_attn(got, "bfloat16", q, hosts, table, cu, kv, 16, 64 ** -0.5, window, (news, window))
+
+
+# ------------------------------------------------------------------------------------------------ errors of others
+def test_an_earlier_calls_error_is_not_taken_for_this_ones():
+    """An error that some other call left with the runtime: the operators run, succeed, and leave it to whoever asks for it."""
+    L = wr.load_library()
+    for f in ("hipSetDevice", "hipGetLastError", "hipPeekAtLastError"):
+        getattr(L, f).restype = C.c_int                            # the runtime the library is linked against, found through it
+    cache, hosts, _, table, q, cu, kv = attn_setup(3, "float16", [20, 5], [1, 1], 2, 1, 64, 16)
+    x, u, tok = dev(np.eye(2, 50, 7, dtype=np.float32) * 50), dev(np.full(2, 0.5, np.float32)), dev(np.full(2, -9, np.int32))
+    rows, slots = dev(np.ones((2, 2, 64), np.float16)), dev(np.full(2, -1, np.int32))
+    out = sv.PagePlan.allocate(2, 4)
+    plan_in = [dev(np.array(v, np.int32)) for v in ([3, 4], [1, 1], [9])]
+    td, qd, od, cud, kvd = dev(table), dev(q, "float16"), dev(np.zeros_like(q), "float16"), dev(cu), dev(kv)
+    calls = [lambda: sv.plan_pages(*plan_in, td, 16, out), lambda: sv.write_kv(cache, rows, rows, slots), lambda: sv.sample_tokens(x, u, tok),
+             lambda: sv.paged_attention(qd, cache, td, cud, kvd, 1, 20, od)]
+    for call in calls:
+        assert L.hipSetDevice(4096) != 0                           # no such device: an error, and nothing else
+        err = L.hipPeekAtLastError()
+        assert err != 0
+        call()
+        assert L.hipPeekAtLastError() == err and L.hipGetLastError() == err and L.hipGetLastError() == 0
+    assert L.wmi_dev_sync() == 0
+    assert tok.numpy().tolist() == [7, 8]
+    check_attn(od.numpy(), "float16", q, hosts, table, cu, kv, 16, 64 ** -0.5)
