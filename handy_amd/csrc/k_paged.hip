@@ -249,6 +249,13 @@ template <class T> struct AttnRef {
     }
 };
 
+// A result in the cache's type. It is a mean of values of V, but the weights above the line are rounded and those below are not: a mean of
+// f16's largest values can pass 65504 by that rounding and stays there. (Infinity and NaN, which V holds itself, go through.)
+template <class T> __device__ __forceinline__ T attn_result(float x) {
+    if constexpr (std::is_same<T, f16>::value) { if (fabsf(x) < INFINITY) x = __builtin_amdgcn_fmed3f(x, -65504.0f, 65504.0f); }
+    return (T)x;
+}
+
 template <class T> __device__ __forceinline__ u16x4 not_finite(typename Mma<T>::V4 v) {
     const u16x4 b = __builtin_bit_cast(u16x4, v);
     return (u16x4)((b & Mma<T>::kExp) == Mma<T>::kExp);                    // all ones where infinite or NaN
@@ -481,7 +488,7 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(PagedAttn a, AttnPar
                 const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;           // a row that sees nothing gives zeros
                 V4 y;
 #pragma unroll
-                for (int r = 0; r < 4; r++) y[r] = (T)(acc[r] * inv);
+                for (int r = 0; r < 4; r++) y[r] = attn_result<T>(acc[r] * inv);
                 *(V4 *)((T *)a.out + orow * a.o_row + oh * a.o_head + e) = y;
             } else {
                 const long at = ((long)part * a.n_rows + orow) * (a.hkv * a.group) + oh;
@@ -731,12 +738,25 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_chunk_kernel(PagedAttn a, At
     if (parts == 1) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         T *dst = (T *)a.out + (rq.q0 + tok) * a.o_row + hq * a.o_head;
+        float big = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            o[b] *= inv;
+#pragma unroll
+            for (int i = 0; i < 16; i++) big = fmaxf(big, fabsf(o[b][i]));
+        }
+        if (std::is_same<T, f16>::value && big > 65504.0f) {               // (attn_result for each costs short prompts 2.5 % instead of 1)
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[b][i] = (float)attn_result<T>(o[b][i]);
+        }
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int e = b * 32 + 8 * i + 4 * h;
-                if (e < a.dim) *(V4 *)(dst + e) = V4{(T)(o[b][4 * i] * inv), (T)(o[b][4 * i + 1] * inv), (T)(o[b][4 * i + 2] * inv), (T)(o[b][4 * i + 3] * inv)};
+                if (e < a.dim) *(V4 *)(dst + e) = V4{(T)o[b][4 * i], (T)o[b][4 * i + 1], (T)o[b][4 * i + 2], (T)o[b][4 * i + 3]};
             }
     } else {
         const long at = ((long)part * a.n_rows + rq.q0 + tok) * (a.hkv * a.group) + hq;
@@ -788,7 +808,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, AttnParts 
     for (int e = 0; e < E; e++) red[wave][lane * E + e] = acc[e];
     __syncthreads();
     l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    if (tid < a.dim) ((T *)a.out)[row * a.o_row + hq * a.o_head + tid] = (T)(((red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid])) * (l == 0.0f ? 0.0f : 1.0f / l));
+    if (tid < a.dim) ((T *)a.out)[row * a.o_row + hq * a.o_head + tid] = attn_result<T>(((red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid])) * (l == 0.0f ? 0.0f : 1.0f / l));
 }
 
 // How a call is cut up. The step kernel takes calls whose requests bring at most 16 packed rows each, as far as the caller says;

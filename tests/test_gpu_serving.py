@@ -725,6 +725,24 @@ def test_attention_windows_as_long_as_they_come_and_more_rows_than_keys(news, wi
     check_attn(got, "bfloat16", q, hosts, table, cu, kv, 16, 64 ** -0.5, window, (news, window))
 
 
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (40, 4)])
+@pytest.mark.parametrize("new,hint", [(1, 0), (1, 1), (60, 0), (60, 1)])
+def test_attention_of_the_largest_values(dim, page, new, hint):
+    """float16 values of 65504 and -65504, the largest there are: a mean of them is one of them, not infinity, whatever the weights' roundings add up
+    to. Bound: the weights' rounding, half a step each."""
+    rng = np.random.default_rng(dim)
+    lens = [3, 2, 700, 17, 1, 5]
+    news = [min(new, L) for L in lens]
+    cache, hosts, _, table, q, cu, kv = attn_setup(11, "float16", lens, news, 2, 2, dim, page)
+    big = np.where(np.arange(dim) % 2 == 0, 65504.0, -65504.0)
+    hosts[1] = np.broadcast_to(big, hosts[1].shape).astype(np.float16)
+    cache = sv.PagedCache(cache.k, dev(hosts[1], "float16"))
+    got = values(run_attn(cache, table, q, cu, kv, "float16", max(news), max(lens) if hint == 0 else hint), "float16")
+    assert np.isfinite(got).all()
+    assert (np.abs(got - big) <= 65504 * 2.0 ** -10).all()
+    del rng
+
+
 # ------------------------------------------------------------------------------------------------ errors of others
 def test_an_earlier_calls_error_is_not_taken_for_this_ones():
     """An error that some other call left with the runtime: the operators run, succeed, and leave it to whoever asks for it."""
