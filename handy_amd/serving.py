@@ -10,6 +10,7 @@ without waiting; outputs are the caller's buffers, so calls can be captured into
 anything is enqueued."""
 import ctypes as C
 import math
+import operator
 import struct
 from typing import Optional
 
@@ -104,6 +105,16 @@ def _dtype(x) -> str:
     return n
 
 
+def _i32(v, name: str):
+    """v where it fits the C ABI's int (ctypes would pass its low bits on)"""
+    try:
+        if -0x80000000 <= operator.index(v) <= 0x7fffffff:
+            return v
+    except TypeError:
+        pass
+    raise ValueError(f"{name}: {v} is no 32-bit whole number")
+
+
 def _flat(x, dtype: str, n: int, name: str):
     """pointer of a contiguous 1-d array of at least n elements (none of no elements)"""
     s = x.shape
@@ -154,7 +165,7 @@ class PagedCache:
         if len(k.shape) != 4 or tuple(k.shape) != tuple(v.shape) or tuple(k.stride()) != tuple(v.stride()) or (k.shape[3] > 1 and k.stride()[3] != 1):
             raise ValueError("K and V: [n_pages, page_tokens, n_kv_heads, head_dim] with the same strides and a contiguous last axis")
         self.k, self.v, self.dtype = k, v, dt
-        self.n_pages, self.page_tokens, self.n_kv_heads, self.head_dim = (int(n) for n in k.shape)
+        self.n_pages, self.page_tokens, self.n_kv_heads, self.head_dim = (int(_i32(n, "K and V")) for n in k.shape)
         st = k.stride()
         self.c = wr.wmi_paged_cache(k.data_ptr(), v.data_ptr(), _DTYPES[dt], self.n_pages, self.page_tokens, self.n_kv_heads, self.head_dim, st[0], st[1], st[2])
         self.ref = C.byref(self.c)
@@ -166,7 +177,7 @@ class PagePlan:
 
     def __init__(self, cu_q, kv_lens, slots, positions, counts):
         self.cu_q, self.kv_lens, self.slots, self.positions, self.counts = cu_q, kv_lens, slots, positions, counts
-        self.n_seq, self.n_rows = int(kv_lens.shape[0]), int(slots.shape[0])
+        self.n_seq, self.n_rows = int(_i32(kv_lens.shape[0], "kv_lens")), int(_i32(slots.shape[0], "slots"))
         self._p = (_flat(cu_q, "int32", self.n_seq + 1, "cu_q"), _flat(kv_lens, "int32", self.n_seq, "kv_lens"), _flat(slots, "int32", self.n_rows, "slots"),
                    _flat(positions, "int32", self.n_rows, "positions"), self.n_rows, _flat(counts, "int32", 4, "counts"))
 
@@ -187,7 +198,7 @@ def plan_pages(ctx_lens, new_lens, free_pages, block_table, page_tokens: int, ou
     if ctx_lens.shape[0] != n_seq or new_lens.shape[0] != n_seq:
         raise ValueError(f"ctx_lens, new_lens: expected the plan's {n_seq} requests")
     rc = _lib().wmi_paged_plan(_flat(ctx_lens, "int32", n_seq, "ctx_lens"), _flat(new_lens, "int32", n_seq, "new_lens"), n_seq,
-                               _flat(free_pages, "int32", n_free, "free_pages"), n_free, page_tokens, tp, cols, stride, *out._p, stream)
+                               _flat(free_pages, "int32", n_free, "free_pages"), _i32(n_free, "free_pages"), _i32(page_tokens, "page_tokens"), tp, cols, stride, *out._p, stream)
     if rc:
         _check(rc, "plan_pages")
     return out
@@ -196,7 +207,7 @@ def plan_pages(ctx_lens, new_lens, free_pages, block_table, page_tokens: int, ou
 def write_kv(cache: PagedCache, k_new, v_new, slots, stream: int = 0) -> None:
     """cache[slots[r]] = k_new[r], v_new[r] (rows [n_kv_heads, head_dim], any row and head strides); rows with a slot outside the cache
     are skipped. The slots of one call must be distinct."""
-    n = k_new.shape[0]
+    n = _i32(k_new.shape[0], "k_new")
     shape = (n, cache.n_kv_heads, cache.head_dim)
     kp, kr, kh = _rows(k_new, shape, cache.dtype, "k_new")
     vp, vr, vh = _rows(v_new, shape, cache.dtype, "v_new")
@@ -207,8 +218,11 @@ def write_kv(cache: PagedCache, k_new, v_new, slots, stream: int = 0) -> None:
 
 def paged_attention_workspace(cache: PagedCache, n_rows: int, n_q_heads: int, n_seq: int, max_new: int = 0, max_kv: int = 0) -> int:
     """Bytes of device memory `paged_attention` needs for these sizes (0: none)."""
-    a = wr.wmi_paged_attn(None, None, None, None, None, 0, 0, 0, 0, 0, 0, n_rows, n_seq, n_q_heads, 0, max_new, max_kv, 1.0)
-    need = _lib().wmi_paged_attention_workspace(cache.ref, C.byref(a))
+    try:
+        a = _ATTN.pack(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, n_rows, n_seq, n_q_heads, 0, max_new, max_kv, 1.0)
+    except struct.error as e:
+        raise ValueError(f"paged_attention_workspace: {e}") from None
+    need = _lib().wmi_paged_attention_workspace(cache.ref, a)
     if need < 0:
         _check(int(need), "paged_attention_workspace")
     return int(need)
@@ -249,7 +263,7 @@ def sample_tokens(logits, uniform, token, logprob=None, temperature=None, top_k=
     dt, shape, st = _DTYPES.get(_dtype(logits), -1), logits.shape, logits.stride()
     if dt < 0 or len(shape) != 2 or (st[1] != 1 and shape[1] > 1):
         raise ValueError("logits: expected float32, float16 or bfloat16 [n_rows, n_vocab] with contiguous rows")
-    n, v = shape
+    n, v = _i32(shape[0], "logits"), _i32(shape[1], "logits")
     rc = _lib().wmi_sample_tokens(
         logits.data_ptr() if n else None, dt, st[0], n, v, _flat(uniform, "float32", n, "uniform"),
         None if temperature is None else _flat(temperature, "float32", n, "temperature"), None if top_k is None else _flat(top_k, "int32", n, "top_k"),

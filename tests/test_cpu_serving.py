@@ -264,3 +264,22 @@ def test_attention_refuses_an_output_that_shares_memory():
     for name in ("q", "out", "block_table", "cu_q", "kv_lens"):
         assert refused(ws=base[name], ws_bytes=need, **long) and refused(ws=base[name] // 16 * 16 - (need - 1) // 16 * 16, ws_bytes=need, **long), name
     assert refused(ws=cache.k, ws_bytes=need, **long) and refused(ws=cache.v, ws_bytes=need, **long) and not refused(ws=0x6000000, ws_bytes=need, **long)
+
+
+def test_sizes_that_do_not_fit_are_value_errors_too():
+    """Whole numbers past 32 bits are errors in every call, not what their low bits say."""
+    cache = sv.PagedCache(Fake((8, 16, 2, 64), "float16"), Fake((8, 16, 2, 64), "float16"))
+    i32 = lambda *s: Fake(s, "int32")
+    plan = sv.PagePlan(i32(4), i32(3), i32(9), i32(9), i32(4))
+    for page in (2 ** 32 + 16, -2 ** 32 + 16, 16.5):
+        with pytest.raises(ValueError):
+            sv.plan_pages(i32(3), i32(3), i32(5), i32(3, 4), page, plan)
+    for kw in (dict(n_rows=2 ** 32 + 1), dict(n_q_heads=2 ** 32 + 2), dict(n_seq=2 ** 32 + 1), dict(max_new=2 ** 32), dict(max_kv=2 ** 40)):
+        with pytest.raises(ValueError):
+            sv.paged_attention_workspace(cache, **{**dict(n_rows=1, n_q_heads=2, n_seq=1, max_new=1, max_kv=9), **kw})
+    with pytest.raises(ValueError):
+        sv.PagedCache(Fake((2 ** 32 + 8, 16, 2, 64), "float16"), Fake((2 ** 32 + 8, 16, 2, 64), "float16"))
+    with pytest.raises(ValueError):
+        sv.sample_tokens(Fake((2 ** 32 + 1, 50), "float32"), Fake((2 ** 32 + 1,), "float32"), i32(2 ** 32 + 1))
+    with pytest.raises(ValueError):
+        sv.write_kv(cache, Fake((2 ** 32 + 1, 2, 64), "float16"), Fake((2 ** 32 + 1, 2, 64), "float16"), i32(2 ** 32 + 1))
