@@ -826,7 +826,8 @@ static AttnShape attn_shape(const PagedAttn &a) {
     const long work = (long)s.tiles * a.hkv, full = s.step ? 2048 : 1024, least = s.step ? kStepLeast * kStepKeys : kChunkLeast * kChunkKeys;
     long n = full / work;
     if (n > keys / least) n = keys / least;
-    s.splits = n < 1 ? 1 : n > kMaxParts ? kMaxParts : (int)n;
+    const bool joinable = (long)a.n_rows * a.hkv * a.group < 1L << 24;     // (the join's 256 threads a pair fit a grid)
+    s.splits = n < 1 || !joinable ? 1 : n > kMaxParts ? kMaxParts : (int)n;
     return s;
 }
 

@@ -283,3 +283,11 @@ def test_sizes_that_do_not_fit_are_value_errors_too():
         sv.sample_tokens(Fake((2 ** 32 + 1, 50), "float32"), Fake((2 ** 32 + 1,), "float32"), i32(2 ** 32 + 1))
     with pytest.raises(ValueError):
         sv.write_kv(cache, Fake((2 ** 32 + 1, 2, 64), "float16"), Fake((2 ** 32 + 1, 2, 64), "float16"), i32(2 ** 32 + 1))
+
+
+def test_split_calls_stay_within_a_grid():
+    """The join of split keys has a workgroup of 256 threads for each row and query head, and a grid holds 2^32 threads: calls of 2^24 pairs and more
+    (rows reserved far beyond the tokens that max_new and n_seq speak of) are not split and need no workspace."""
+    L = wr.load_library()
+    need = lambda rows: L.wmi_paged_attention_workspace(C.byref(cache_struct()), C.byref(attn_struct(n_rows=rows, n_seq=4, max_new=1, max_kv=10 ** 6)))
+    assert need(2 ** 22 - 1) > 0 and need(2 ** 22) == 0 and need(2 ** 28 - 1) == 0
