@@ -606,6 +606,17 @@ WHISPER_API int wmi_sample_tokens(const void *logits, int dtype, long long row_s
     if (n_vocab > kDrawMaxVocab) return -3;
     if (n_rows == 0) return 0;
     if (!logits || !uniform || !token || ((uintptr_t)logits & (dtype == WMI_F32 ? 3 : 1))) return -1;
+    // Rows are drawn by workgroups of their own, each of which reads its entry of every array before it writes its outputs: those may lie in
+    // place of a parameter's, and nowhere else among what is read.
+    auto meet = [](const void *a, long long a_bytes, const void *b, long long b_bytes) { return (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes; };
+    const long long each = 4LL * n_rows, all = ((n_rows - 1) * row_stride + n_vocab) * (dtype == WMI_F32 ? 4 : 2);
+    if (logprob && meet(token, each, logprob, each)) return -1;
+    for (const void *out : {(const void *)token, (const void *)logprob}) {
+        if (!out) continue;
+        if (meet(out, each, logits, all)) return -1;
+        for (const void *in : {(const void *)uniform, (const void *)temperature, (const void *)top_k, (const void *)top_p, (const void *)min_p})
+            if (in && in != out && meet(out, each, in, each)) return -1;
+    }
     hipStream_t st = (hipStream_t)stream;
     const ServeCall call(st);
     if (!call.ok()) return -4;

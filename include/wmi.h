@@ -342,7 +342,8 @@ WHISPER_API int wmi_paged_attention(const wmi_paged_cache *cache, const wmi_page
  * NULL (temperature 1, filter off); per row top_k <= 0, top_p >= 1, min_p <= 0 turn a filter off. -infinity and NaN are never
  * drawn; a row with nothing to draw gives token -1. logprob (may be NULL): logarithm of the token's probability at this
  * temperature (at 1 when temperature <= 0) before the filters. Masses are sums in 64-bit whole numbers: the result does not
- * depend on anything but the row. n_vocab <= 262144. */
+ * depend on anything but the row. token and logprob may lie in place of a parameter array, entry by entry, and share no other memory with
+ * the inputs or each other (-1). n_vocab <= 262144. */
 WHISPER_API int wmi_sample_tokens(const void *logits, int dtype, long long row_stride, int n_rows, int n_vocab, const float *uniform, const float *temperature,
                                   const int *top_k, const float *top_p, const float *min_p, int *token, float *logprob, void *stream);
 

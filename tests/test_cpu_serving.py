@@ -291,3 +291,25 @@ def test_split_calls_stay_within_a_grid():
     L = wr.load_library()
     need = lambda rows: L.wmi_paged_attention_workspace(C.byref(cache_struct()), C.byref(attn_struct(n_rows=rows, n_seq=4, max_new=1, max_kv=10 ** 6)))
     assert need(2 ** 22 - 1) > 0 and need(2 ** 22) == 0 and need(2 ** 28 - 1) == 0
+
+
+def test_draws_refuse_outputs_that_share_memory():
+    """token and logprob may take the place of a parameter array entry by entry (a row reads its own before it writes), and share memory with
+    nothing else. Told from the codes without a GPU: -1 for the arguments, -4 for a call whose arguments are in order."""
+    L = wr.load_library()
+    base = dict(x=0x1000000, u=0x2000000, T=0x2100000, k=0x2200000, p=0x2300000, m=0x2400000, tok=0x2500000, lp=0x2600000)
+
+    def call(rows=5, V=50, stride=64, **kw):
+        a = {**base, **kw}
+        return L.wmi_sample_tokens(a["x"], 2, stride, rows, V, a["u"], a["T"], a["k"], a["p"], a["m"], a["tok"], a["lp"], None)
+    if call() != -4:
+        pytest.skip("a GPU is present: these addresses are refused as no memory of it")
+    for out in ("tok", "lp"):
+        for name in ("u", "T", "k", "p", "m"):
+            assert call(**{out: base[name]}) == -4 and call(**{out: base[name] + 4}) == -1 and call(**{out: base[name] - 16}) == -1 and call(**{out: base[name] + 20}) == -4, (out, name)
+        end = base["x"] + (4 * 64 + 50) * 4
+        assert call(**{out: base["x"]}) == -1 and call(**{out: end - 4}) == -1 and call(**{out: end}) == -4 and call(**{out: base["x"] - 20}) == -4
+        assert call(rows=1, stride=0, **{out: base["x"] + 50 * 4}) == -4 and call(rows=3, stride=0, **{out: base["x"] + 49 * 4}) == -1
+    for d in (0, 4, -16):
+        assert call(lp=base["tok"] + d) == -1
+    assert call(lp=base["tok"] + 20) == -4 and call(lp=None, T=None, k=None, p=None, m=None) == -4

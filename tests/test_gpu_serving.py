@@ -725,6 +725,20 @@ def test_attention_windows_as_long_as_they_come_and_more_rows_than_keys(news, wi
     check_attn(got, "bfloat16", q, hosts, table, cu, kv, 16, 64 ** -0.5, window, (news, window))
 
 
+def test_draws_into_the_parameters_own_arrays():
+    """token in place of top_k, logprob in place of the uniform numbers or the temperatures: the results of separate arrays."""
+    rng = np.random.default_rng(4)
+    for rows, V in ((700, 300), (300, 20000), (9, 30000)):
+        x, u = (rng.standard_normal((rows, V)) * 3).astype(np.float32), rng.random(rows).astype(np.float32)
+        x[rows // 2] = -np.inf
+        T, k = rng.uniform(0.3, 1.2, rows).astype(np.float32), rng.integers(1, 50, rows).astype(np.int32)
+        tok, lp = run_sample(x, "float32", u, T, k)
+        for place in ("u", "T"):
+            ud, Td, kd = dev(u), dev(T), dev(k)
+            sv.sample_tokens(dev(x), ud, kd, logprob=ud if place == "u" else Td, temperature=Td, top_k=kd)
+            assert np.array_equal(kd.numpy(), tok) and np.array_equal((ud if place == "u" else Td).numpy(), lp)
+
+
 @pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (40, 4)])
 @pytest.mark.parametrize("new,hint", [(1, 0), (1, 1), (60, 0), (60, 1)])
 def test_attention_of_the_largest_values(dim, page, new, hint):
