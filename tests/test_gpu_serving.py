@@ -780,3 +780,94 @@ def test_an_earlier_calls_error_is_not_taken_for_this_ones():
     assert L.wmi_dev_sync() == 0
     assert tok.numpy().tolist() == [7, 8]
     check_attn(od.numpy(), "float16", q, hosts, table, cu, kv, 16, 64 ** -0.5)
+
+
+# ------------------------------------------------------------------------------------------------ attention: every kernel's holes and masks
+def upload(base, host, dtype):
+    a = np.ascontiguousarray(host)
+    assert wr.load_library().wmi_dev_upload(base.data_ptr(), a.ctypes.data, a.nbytes) == 0
+
+
+def junk_of(dtype):
+    return (np.float16(np.inf), np.float16(np.nan)) if dtype == "float16" else (np.uint16(0x7F80), np.uint16(0x7FC0))
+
+
+KERNELS = [([1, 1, 1], None), ([5, 1, 3], None), ([40, 70, 9], None), ([40, 70, 9], 0)]      # new tokens, max_kv hint: step, step or chunk, chunk of 4 waves, of 8 (dims above 64)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim", [40, 64, 80, 128])
+@pytest.mark.parametrize("page", [1, 8, 16, 64])
+def test_attention_of_every_kernel_ignores_what_no_row_sees(dtype, dim, page):
+    """Stale memory (NaN, infinity) in unused slots and pages, and table entries that name no page, at every head dim, page size and type, for
+    the step kernel and both chunk kernels, with and without a window."""
+    lens = [203, 150, 77]
+    for news, hint in KERNELS:
+        cache, hosts, bases, table, q, cu, kv = attn_setup(dim + page, dtype, lens, news, 2, 4, dim, page)
+        seen = np.zeros(hosts[0].shape[:2], bool)
+        for i, L in enumerate(lens):
+            seen[table[i, np.arange(L) // page], np.arange(L) % page] = True
+        clean = [np.where(seen[:, :, None, None], h, np.zeros((), h.dtype)) for h in hosts]
+        wrong = table.copy()
+        last = [(L - 1) // page for L in lens]
+        wrong[0, last[0] // 3], wrong[1, 0], wrong[1, last[1] // 2], wrong[2, last[2]] = -1, hosts[0].shape[0], 2 ** 31 - 1, -(2 ** 31)
+        for junk in (junk_of(dtype), junk_of(dtype)[::-1]):
+            for h, base, j in zip(hosts, bases, junk):
+                h[~seen] = j
+                upload(base, h, dtype)
+            for tb in (table, wrong):
+                for window in (0, 20):
+                    got = run_attn(cache, tb, q, cu, kv, dtype, max(news), max(lens) if hint is None else hint, window=window)
+                    check_attn(got, dtype, q, clean, tb, cu, kv, page, dim ** -0.5, window, (news, hint, window))
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim,page", [(40, 8), (64, 16), (80, 1), (128, 64), (128, 2)])
+def test_attention_of_every_kernel_keeps_a_bad_value_to_the_rows_that_see_it(dtype, dim, page):
+    """NaN and infinity in the V of a key that some rows of a tile see and others, masked by position or window, do not: the others' results are
+    those of a finite value there."""
+    lens = [203, 150, 77]
+    for news, hint in KERNELS[1:]:
+        cache, hosts, bases, table, q, cu, kv = attn_setup(dim + page, dtype, lens, news, 2, 4, dim, page)
+        at = [L - n // 2 - 1 for L, n in zip(lens, news)]          # seen by the later half of the request's new tokens, up to the window's length on
+        for window in (0, 11):
+            pos = np.concatenate([L - n + np.arange(n) for L, n in zip(lens, news)])
+            bad = np.repeat(at, news)
+            sees = (pos >= bad) & ((pos < bad + window) if window else True)
+            for junk in junk_of(dtype):
+                spoiled = hosts[1].copy()
+                for i, j in enumerate(at):
+                    spoiled[table[i, j // page], j % page] = junk
+                upload(bases[1], spoiled, dtype)
+                got = run_attn(cache, table, q, cu, kv, dtype, max(news), max(lens) if hint is None else hint, window=window)
+                ref = got.copy()
+                zero = hosts[1].copy()
+                for i, j in enumerate(at):
+                    zero[table[i, j // page], j % page] = 0
+                upload(bases[1], zero, dtype)
+                plain = run_attn(cache, table, q, cu, kv, dtype, max(news), max(lens) if hint is None else hint, window=window)
+                check_attn(plain, dtype, q, [hosts[0], zero], table, cu, kv, page, dim ** -0.5, window, (news, hint, window))
+                assert np.array_equal(ref[~sees], plain[~sees]), (news, hint, window)
+                assert sees.any() and not np.isfinite(values(ref, dtype)[sees]).any(), (news, hint, window)
+
+
+WIDE = [
+    # lens, news, hkv, group, dim, page, window: 256 packed rows and more, for the eight-wave chunk kernel
+    ([500, 130, 260], [200, 1, 129], 2, 4, 128, 64, 0),
+    ([600, 90, 333], [150, 90, 7], 2, 2, 128, 16, 50),
+    ([300, 5, 0, 140], [100, 5, 0, 140], 1, 3, 96, 8, 0),
+    ([300, 64, 421], [60, 64, 200], 2, 5, 72, 32, 33),
+    ([257], [257], 1, 33, 128, 128, 0),
+    ([90, 200], [120, 300], 1, 7, 80, 4, 100),                 # more new tokens than keys
+]
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("case", range(len(WIDE)))
+@pytest.mark.parametrize("max_kv", [0, 9000])
+def test_attention_on_eight_waves_matches_restatement(case, dtype, max_kv):
+    lens, news, hkv, group, dim, page, window = WIDE[case]
+    cache, hosts, bases, table, q, cu, kv = attn_setup(case, dtype, lens, news, hkv, group, dim, page, head_major=case % 2 == 0, spread=1.5)
+    assert dim > 64 and max(news) * group >= 256
+    got = run_attn(cache, table, q, cu, kv, dtype, max(news), max_kv, window=window, extra_rows=3)
+    check_attn(got, dtype, q, hosts, table, cu, kv, page, dim ** -0.5, window, str(case))
