@@ -579,13 +579,13 @@ __global__ __launch_bounds__(TH, 4) void draw_kernel(DrawArgs a) {
     }
 }
 
+// Threads of a row. Short rows: four waves, so that more rows share a compute unit. Else sixteen if every row has a compute unit of its
+// own (256), or eight, two rows a compute unit, whose waits then fall under the other's arithmetic (1024 rows of 51866 entries: 99 us
+// against 125). Longer rows take sixteen again: a thread's share is long enough (600 rows of 262144: 317 us against 360).
+static int draw_threads(int n_rows, int n_vocab) { return n_vocab <= 16384 ? 256 : n_rows > 256 && n_vocab <= 131072 ? 512 : 1024; }
 template <class T> static bool draw_launch(const DrawArgs &a, hipStream_t st) {
-    // Short rows: four waves a row, so that more rows share a compute unit. Else sixteen if every row has a compute unit of its own
-    // (256), or eight, two rows a compute unit, whose waits then fall under the other's arithmetic (1024 rows of 51866 entries: 99 us
-    // against 125). Longer rows take sixteen again: a thread's share is long enough (600 rows of 262144: 317 us against 360).
-    if (a.n_vocab <= 16384) return serve_launch(draw_kernel<T, 256>, dim3(a.n_rows), dim3(256), 0, st, a);
-    if (a.n_rows > 256 && a.n_vocab <= 131072) return serve_launch(draw_kernel<T, 512>, dim3(a.n_rows), dim3(512), 0, st, a);
-    return serve_launch(draw_kernel<T, 1024>, dim3(a.n_rows), dim3(1024), 0, st, a);
+    const int th = draw_threads(a.n_rows, a.n_vocab);
+    return serve_launch(th == 256 ? draw_kernel<T, 256> : th == 512 ? draw_kernel<T, 512> : draw_kernel<T, 1024>, dim3(a.n_rows), dim3(th), 0, st, a);
 }
 
 bool draw_tokens(const DrawArgs &a, hipStream_t st) {
@@ -605,6 +605,7 @@ WHISPER_API int wmi_sample_tokens(const void *logits, int dtype, long long row_s
     if (n_rows < 0 || n_vocab < 1 || row_stride < 0 || (dtype != WMI_F16 && dtype != WMI_BF16 && dtype != WMI_F32)) return -1;
     if (n_vocab > kDrawMaxVocab) return -3;
     if (n_rows == 0) return 0;
+    if ((long long)n_rows * draw_threads(n_rows, n_vocab) > 0xffffffffLL) return -3;      // threads of a grid
     if (!logits || !uniform || !token || ((uintptr_t)logits & (dtype == WMI_F32 ? 3 : 1))) return -1;
     // Rows are drawn by workgroups of their own, each of which reads its entry of every array before it writes its outputs: those may lie in
     // place of a parameter's, and nowhere else among what is read.

@@ -338,12 +338,13 @@ WHISPER_API int wmi_paged_attention(const wmi_paged_cache *cache, const wmi_page
  * distribution's logarithm, the tokens are ordered by x, equal ones by index, and kept while their rank is below top_k, the mass
  * before them is below top_p times the mass of the first top_k, and their probability is at least min_p times the largest; the
  * first is always kept. The token is the first, in the vocabulary's order, at which the running mass of the kept ones exceeds
- * uniform (in [0, 1); NaN and less count as 0, more as 1 - 2^-24) times their whole mass. temperature <= 0: the most probable token (lowest index). A parameter array may be
- * NULL (temperature 1, filter off); per row top_k <= 0, top_p >= 1, min_p <= 0 turn a filter off. -infinity and NaN are never
- * drawn; a row with nothing to draw gives token -1. logprob (may be NULL): logarithm of the token's probability at this
- * temperature (at 1 when temperature <= 0) before the filters. Masses are sums in 64-bit whole numbers: the result does not
- * depend on anything but the row. token and logprob may lie in place of a parameter array, entry by entry, and share no other memory with
- * the inputs or each other (-1). n_vocab <= 262144. */
+ * uniform (in [0, 1); NaN and less count as 0, more as 1 - 2^-24) times their whole mass. temperature <= 0: the most probable
+ * token (lowest index). A parameter array may be NULL (temperature 1, filter off); per row top_k <= 0, top_p >= 1, min_p <= 0 turn
+ * a filter off. -infinity and NaN are never drawn; a row with nothing to draw gives token -1. logprob (may be NULL): logarithm of
+ * the token's probability at this temperature (at 1 when temperature <= 0) before the filters. Masses are sums in 64-bit whole
+ * numbers: the result does not depend on anything but the row. token and logprob may lie in place of a parameter array, entry by
+ * entry, and share no other memory with the inputs or each other (-1). n_vocab <= 262144; n_rows < 2^24 up to a vocabulary of
+ * 16384, < 2^23 up to 131072, < 2^22 above (-3). */
 WHISPER_API int wmi_sample_tokens(const void *logits, int dtype, long long row_stride, int n_rows, int n_vocab, const float *uniform, const float *temperature,
                                   const int *top_k, const float *top_p, const float *min_p, int *token, float *logprob, void *stream);
 

@@ -313,3 +313,12 @@ def test_draws_refuse_outputs_that_share_memory():
     for d in (0, 4, -16):
         assert call(lp=base["tok"] + d) == -1
     assert call(lp=base["tok"] + 20) == -4 and call(lp=None, T=None, k=None, p=None, m=None) == -4
+
+
+def test_draws_of_more_rows_than_a_grid_holds_are_refused():
+    """A row is a workgroup of 256 threads (vocabularies up to 16384) to 1024, and a grid holds 2^32 threads."""
+    L = wr.load_library()
+    call = lambda rows, V: L.wmi_sample_tokens(P, 0, V, rows, V, 1 << 50, None, None, None, None, 1 << 51, None, None)
+    for V, most in ((1, 2 ** 24), (16384, 2 ** 24), (16385, 2 ** 23), (131072, 2 ** 23), (131073, 2 ** 22)):
+        assert call(most, V) == -3 and call(2 ** 31 - 1, V) == -3, V
+        assert call(most - 1, V) in (-1, -4), V                    # (no GPU, or no memory of it)
