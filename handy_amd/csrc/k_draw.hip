@@ -7,8 +7,9 @@ namespace wmi {
 
 // Weights w_i = exp((x_i - max x) / T) lie in [0, 1]. They are computed in 64 bits and rounded to whole numbers of 2^-45: sums of up to
 // 2^18 of them fit 64 bits and are exact, so they do not depend on the order in which they are made (nor on which workgroup shape
-// made them), and every comparison of running masses (top-p's border, the draw) is exact. What the rounding of a weight costs is
-// 2^-46 of the largest one: a draw nearer than that to a border may fall on its other side.
+// made them), and neither do the comparisons of running masses (top-p's border, the draw). Rounded are a weight, by 2^-46 of the largest
+// one, and the two products that masses are compared with, top_p and the uniform number times a mass, by 2^-52 of themselves: a draw nearer
+// than that to a border may fall on its other side.
 // The filters keep a prefix of the order (x descending, index ascending). It is described by a value, the cut: entries above it are
 // kept, and of the entries equal to it the first few by index.
 // One workgroup a row; the row comes from HBM once and out of the caches in later passes:
