@@ -140,12 +140,12 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
 //                        running maximum) fill the rest. Prompts of up to 224 tokens, 64 x 20 heads x 64, f16: 33 us, bound by the chain
 //                        lengths - table - keys - two to four tiles in each short-lived workgroup.
 // The keys of a tile of rows may be split over workgroups; paged_join_kernel adds the parts up.
-// A probability is 2^(score c - m), c = |scale| log2(e); its row's reference m moves only when a score passes m + kBias by more than kMove, so
-// that the accumulators are rescaled rarely instead of every tile. m is a whole number: rescaling and joining multiply by powers of two, and a
-// probability's rounding to the cache's type (for the product with V; the sums are of the unrounded ones) does not depend on where its
-// row's reference lies. kBias puts f16's range above 1 to use: the largest probability of a row lies near 2^11 and none reaches 2^16, so
-// that weights down to 2^-25 of the largest keep 11 bits and those down to 2^-36 fewer (with kBias 0 a long tail behind one key 17 nats
-// above it came out 44 % too large). bf16 holds 8 bits whatever the size.
+// A probability is 2^(score c - m), c = |scale| log2(e). Its row's reference m is set by a largest score so far, whose own probability is 2^kBias
+// then, and moves only when a score passes it by more than kMove (in powers of two), so that the accumulators are rescaled rarely instead of
+// every tile. Probabilities are rounded to the cache's type for the product with V, their sums are of the unrounded ones (sums of the
+// rounded ones: the same error, chunks 8 % slower). kBias puts f16's range above 1 to use: no probability reaches 2^16, and weights
+// down to 2^-25 of the largest keep 11 bits, those down to 2^-36 fewer (with kBias 0 a long tail behind one key 17 nats above it came out 44 %
+// too large). bf16 holds 8 bits whatever the size.
 // (Chunks of 4096, f16, 128 dims: 5.82 ms with kMove + kBias = 4 + 11, 5.74 with 8 + 7, 5.90 with 2 + 13; single tokens and 64 dims do not tell
 // them apart.)
 typedef __bf16 bf16;
@@ -243,7 +243,7 @@ template <class T> struct AttnRef {
         const float was = at(c), mx = top * c;
         const bool big = fabsf(mx) >= 0x1p20f;
         base = big ? top : 0.0f;
-        sub = (big ? 0.0f : ceilf(mx)) - Mma<T>::kBias;
+        sub = (big ? 0.0f : mx) - Mma<T>::kBias;
         limit = big ? top : (sub + (Mma<T>::kBias + Mma<T>::kMove)) / c;
         return __builtin_amdgcn_exp2f(was - at(c));
     }

@@ -687,6 +687,30 @@ def test_attention_of_scores_of_any_finite_size(dtype, dim, page, new, sign):
         assert (np.abs(got - ref) <= 3.01 * HALF_STEP[dtype] * np.abs(ref)).all(), (hint, float(np.abs(got / ref - 1).max()))
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (40, 4)])
+@pytest.mark.parametrize("new", [1, 60])
+def test_attention_over_one_key_is_its_value(dtype, dim, page, new):
+    """A row that sees one key gives that key's V to the bit (its weight is 1), and so does one whose other keys are far below it."""
+    lens = [1, 60, 200]
+    news = [min(new, L) for L in lens]
+    cache, hosts, bases, table, q, cu, kv = attn_setup(2, dtype, lens, news, 2, 3, dim, page)
+    got = run_attn(cache, table, q, cu, kv, dtype, max(news), max(lens), window=1)
+    rows = [(i, L - n + t) for i, (L, n) in enumerate(zip(lens, news)) for t in range(n)]
+    own = np.stack([hosts[1][table[i, p // page], p % page] for i, p in rows])
+    assert np.array_equal(got, np.repeat(own, 3, axis=1))
+    first = run_attn(cache, table, q, cu, kv, dtype, max(news), max(lens))
+    at = [r for r, (_, p) in enumerate(rows) if p == 0]
+    assert at and np.array_equal(first[at], np.repeat(own[at], 3, axis=1))
+    k = values(hosts[0], dtype)                                    # every key but the first of its request 100 nats below it
+    k[:] = -50.0 / dim ** 0.5
+    for i in range(len(lens)):
+        k[table[i, 0], 0] *= -1.0
+    upload(bases[0], host_form(k, dtype), dtype)
+    got = run_attn(cache, table, host_form(np.ones(q.shape), dtype), cu, kv, dtype, max(news), max(lens))
+    assert np.array_equal(got, np.repeat(np.stack([hosts[1][table[i, 0], 0] for i, _ in rows]), 3, axis=1))
+
+
 # ------------------------------------------------------------------------------------------------ attention: infinite keys
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
 @pytest.mark.parametrize("dim,page", [(40, 16), (64, 16), (80, 64), (128, 32), (72, 2)])
