@@ -133,11 +133,12 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
 // The query rows of a request's tokens and of the heads that share a key head are packed into one list, row r = token * group +
 // head, so that every K and V byte is read once for all of them.
 //   paged_step_kernel    up to 16 packed rows (single tokens): bound by HBM. Each wave streams its own 16-key tiles. 64 requests of up
-//                        to 8192 keys, 32/8 heads x 128, bf16: 182 us, 6.3 TB/s; 3 of 90 000 - 131 000 keys: 216 us, 6.7 TB/s.
+//                        to 8192 keys, 32/8 heads x 128, bf16, with the join: 190 - 209 us, 5.5 - 6.0 TB/s; 3 of 90 000 - 131 000 keys, f16:
+//                        208 - 234 us, 6.2 - 6.9 TB/s (ranges over sessions; a pure read stream reaches 7.2).
 //   paged_chunk_kernel   128 or 256 packed rows a workgroup, 64-key tiles shared by its waves. Three chunks of about 3800 tokens behind
-//                        20 000 - 28 500 cached ones, 32/8 heads x 128, bf16: 5.2 ms, 1030 TFLOP/s; bound by issue: the matrix pipes are
-//                        busy 44 % of the CU cycles, the vector instructions between two products (exponentials, conversions, the
-//                        running maximum) fill the rest. Prompts of up to 224 tokens, 64 x 20 heads x 64, f16: 33 us, bound by the chain
+//                        20 000 - 28 500 cached ones, 32/8 heads x 128, bf16: 4.9 - 5.7 ms, 940 - 1090 TFLOP/s; bound by issue: the matrix
+//                        pipes are busy 43 % of the CU cycles, the vector instructions between two products (exponentials, conversions, the
+//                        running maximum) fill the rest. Prompts of up to 224 tokens, 64 x 20 heads x 64, f16: 32 us, bound by the chain
 //                        lengths - table - keys - two to four tiles in each short-lived workgroup.
 // The keys of a tile of rows may be split over workgroups; paged_join_kernel adds the parts up.
 // A probability is 2^(score c - m), c = |scale| log2(e). Its row's reference m is set by a largest score so far, whose own probability is 2^kBias
