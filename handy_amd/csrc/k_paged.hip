@@ -233,7 +233,8 @@ struct AttnParts { float *o; float2 *ml; int splits; };
 
 // A row's reference while its keys go by. Where score * c is 2^20 or more, the rounded product that a reference is made of and the fma in
 // the exponent part by a tenth of a power of two and more (from 2^28 on by more than the type's range: finite scores gave NaN, or zeros).
-// Such a row takes its largest score off first, which leaves the largest ones exact; the products then only scale what is summed up already.
+// Such a row takes its largest score off first, which leaves the largest ones exact; the products then only scale what is summed up already
+// (and have to be finite themselves).
 template <class T> struct AttnRef {
     float limit = -INFINITY;                               // scores above it move the reference (-infinity: none seen)
     float sub = 0.0f, base = 0.0f;                         // exponents are (score - base) c - sub; base 0: sub is the reference

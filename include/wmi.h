@@ -70,8 +70,8 @@ WHISPER_API void wmi_set_beam_candidates_sampled(struct whisper_state *state, in
  * wmi_sample_tokens' kernel instead of on the host: no probability rows cross the bus (207 KB a sequence and token for a
  * 51 866-entry vocabulary), and top_k (0: off), top_p (1: off) and min_p (0: off) narrow them down. Every sequence still draws from
  * its own mt19937 (one number a token, not two), so the transcripts at a temperature are others than with the host's draws, and the
- * same on every run; a token's log-probability is the host draw's: relative to all that the rules left before the one on timestamps. Best of five at T = 0.6 on large-v3-turbo, 32 clips:
- * 118 ms instead of 500. Off by default. Returns 0, -1 for bad arguments. */
+ * same on every run; a token's log-probability is the host draw's: relative to all that the rules left before the one on
+ * timestamps. Best of five at T = 0.6 on large-v3-turbo, 32 clips: 118 ms instead of 500. Off by default. Returns 0, -1 for bad arguments. */
 WHISPER_API int wmi_set_device_draws(struct whisper_state *state, int on, int top_k, float top_p, float min_p);
 /* on != 0: decoder passes that feed several tokens of a sequence (prompts with text context, whisper_decode of more than one
  * token) use wmi_paged_attention's kernels for the self-attention of all their rows: the rows of a sequence share the keys they
